@@ -770,7 +770,7 @@ __device__ __forceinline__ void fetch_row(cfloat_p head, cdouble_p stats, long l
     if (stats) { o.mean = stats[2 * r]; o.m2 = stats[2 * r + 1]; }
 }
 
-typedef float v2f __attribute__((ext_vector_type(2)));   // two adjacent columns: one v_pk_fma_f32 per pair
+typedef float v2f __attribute__((ext_vector_type(2)));   // two adjacent columns (two v_fma_f32: the build keeps packed fp32 off)
 
 // ReLU + LayerNorm moments of one full row of 256 (float4 per lane, every lane valid)
 __device__ __forceinline__ void row_stats_full(const float (&a)[4], float eps, float& mean, float& rstd) {
@@ -789,8 +789,8 @@ __device__ __forceinline__ void env_row_z(const RowIn<EnvIn<NR>::HD>& row, const
                                           const bool has_stats, float invD, float eps_in, const float (&sv)[4],
                                           const float (&cv)[4], float (&zr)[4], float& mean_in, float& rstd_in) {
     constexpr int HD = EnvIn<NR>::HD;
-    // the column pairs are explicit 2-vectors: left to itself the vectoriser pairs over k for part of the loop (a
-    // v_pk_mul + 2 adds per pair) and leaves the rest scalar -- 88 VALU instructions per row instead of 36
+    // the column pairs are explicit 2-vectors, so that every product stays one multiply-add (with packed fp32 on, the vectoriser paired
+    // over k for part of the loop)
     v2f u0 = {0.f, 0.f}, u1 = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < HD; ++k) {
