@@ -6,6 +6,8 @@
 `relu_ln_head(...)`   the last block's tail fused with the narrow Linear after it (Gaussian mean, value head).
 `actor_l1(...)`       the actor's whole first block from the compact features (structured.py) -- the pre-activation
                       never reaches memory in either direction.
+`gated_delta(...)`    the gated delta rule over a sequence, with its gradient (include/dcc_delta.h): the memory layer of the
+                      recurrent policies (rnn.py).
 All fall back to the plain torch formulation when the tensors are not float32 CUDA tensors (CPU tests,
 autocast) or the shape has no compiled variant; on a GPU box the library itself must load (dcc_hip raises).
 """
@@ -283,3 +285,67 @@ def value_loss(values, value_preds, returns, active, norm, clip, huber_delta, us
     return _ValueLoss.apply(values, value_preds, returns, active, norm, float(clip),
                             float(huber_delta) if huber_delta is not None else -1.0, bool(use_clipped), bool(use_masks),
                             int(n_agents))
+
+
+class _GatedDelta(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, masks, scale):
+        import dcc_hip
+        last_contiguous = lambda x: x if x.shape[-1] == 1 or x.stride(-1) == 1 else x.contiguous()
+        q, k, v = last_contiguous(q), last_contiguous(k), last_contiguous(v)
+        train = any(ctx.needs_input_grad)
+        o, last, ckpt = dcc_hip.gated_delta_fwd(q, k, v, g, beta, None if state is None else state.contiguous(), masks, scale, want_ckpt=train)
+        if train:
+            ctx.save_for_backward(q, k, v, g, beta, masks, ckpt)
+            ctx.scale = scale
+            ctx.set_materialize_grads(False)
+        return o, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dlast):
+        import dcc_hip
+        q, k, v, g, beta, masks, ckpt = ctx.saved_tensors
+        if do is None and dlast is None:
+            return (None,) * 8
+        if do is None:
+            do = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
+        if do.shape[-1] > 1 and do.stride(-1) != 1:
+            do = do.contiguous()
+        dq, dk, dv, dg, db, ds = dcc_hip.gated_delta_bwd(q, k, v, g, beta, masks, ctx.scale, ckpt, do,
+                                                         None if dlast is None else dlast.contiguous())
+        return dq, dk, dv, dg, db, ds if ctx.needs_input_grad[5] else None, None, None
+
+
+def _gated_delta_torch(q, k, v, g, beta, state, masks, scale):
+    """The recurrence token by token in plain torch (host logic on the CPU, double precision, autocast)."""
+    T, B, H, DV = v.shape
+    rep, DK = H // q.shape[2], q.shape[3]
+    acc = torch.promote_types(v.dtype, torch.float32)
+    heads = lambda x: x.to(acc).repeat_interleave(rep, dim=1)
+    S = torch.zeros(B, H, DK, DV, dtype=acc, device=v.device) if state is None else state.to(acc)
+    outs = []
+    for t in range(T):
+        S = S * g[t].to(acc).exp().view(B, H, 1, 1)
+        if masks is not None:
+            S = torch.where(masks[t].view(B, 1, 1, 1) == 0, torch.zeros((), dtype=acc, device=v.device), S)
+        kt = heads(k[t]).unsqueeze(-1)
+        u = beta[t].to(acc).unsqueeze(-1) * (v[t].to(acc) - (S * kt).sum(-2))
+        S = S + kt * u.unsqueeze(-2)
+        outs.append((S * heads(q[t]).unsqueeze(-1)).sum(-2) * scale)
+    o = torch.stack(outs) if outs else v.new_zeros(v.shape).to(acc)
+    return o.to(v.dtype), S
+
+
+def gated_delta(q, k, v, g, beta, state=None, masks=None, scale=None):
+    """Gated delta rule over T tokens, differentiable in q, k, v, g, beta and state.  Per row b and head h, with a state S [DK, DV]:
+        S' = m_t exp(g_t) S;   u = beta_t (v_t - S'^T k_t);   S = S' + k_t u^T;   o_t = scale * S^T q_t
+    q, k [T,B,HK,DK], v [T,B,H,DV] (value head h reads key head h // (H // HK)), g, beta [T,B,H], state [B,H,DK,DV] or None (zero),
+    masks [T,B] or None (0: the state restarts from zero before that token).  -> o [T,B,H,DV], last state [B,H,DK,DV].
+    On the GPU float32 / bfloat16 / float16 q, k, v with float32 g, beta, state run the HIP kernels."""
+    if q.dim() != 4 or v.dim() != 4:
+        raise ValueError("gated_delta: q, k are [T,B,HK,DK] and v is [T,B,H,DV]")
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if v.is_cuda and v.dtype in (torch.float32, torch.bfloat16, torch.float16) and not torch.is_autocast_enabled():
+        return _GatedDelta.apply(q, k, v, g, beta, state, masks, scale)
+    return _gated_delta_torch(q, k, v, g, beta, state, masks, scale)

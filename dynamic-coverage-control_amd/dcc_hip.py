@@ -44,13 +44,28 @@ class ObsFeat(ctypes.Structure):       # include/dcc_env.h: dcc_obs_feat
     _fields_ = [("head", _vp), ("poi_feat", _vp), ("stats", _vp), ("cstats", _vp), ("xa", _vp), ("xc", _vp)]
 
 
+class DeltaSeq(ctypes.Structure):      # include/dcc_delta.h: dcc_delta_seq
+    _fields_ = [("T", ctypes.c_int64), ("B", ctypes.c_int64), ("HK", ctypes.c_int32), ("H", ctypes.c_int32), ("DK", ctypes.c_int32),
+                ("DV", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", ctypes.c_float), ("q", _vp), ("k", _vp), ("v", _vp),
+                ("g", _vp), ("beta", _vp), ("masks", _vp), ("state0", _vp), ("st_q", ctypes.c_int64 * 3), ("st_k", ctypes.c_int64 * 3),
+                ("st_v", ctypes.c_int64 * 3), ("st_g", ctypes.c_int64 * 3), ("st_beta", ctypes.c_int64 * 3),
+                ("st_masks", ctypes.c_int64 * 2), ("o", _vp), ("state1", _vp), ("ckpt", _vp)]
+
+
+class DeltaGrad(ctypes.Structure):     # include/dcc_delta.h: dcc_delta_grad
+    _fields_ = [("dout", _vp), ("st_do", ctypes.c_int64 * 3), ("dstate1", _vp), ("ckpt", _vp), ("dq", _vp), ("dk", _vp), ("dv", _vp),
+                ("dg", _vp), ("dbeta", _vp), ("dstate0", _vp)]
+
+
 EXPORTS = ["dcc_obs_expand", "dcc_gae_compute", "dcc_returns_compute", "dcc_abi_version", "dcc_last_error", "dcc_env_cfg_default", "dcc_env_create", "dcc_env_destroy",
            "dcc_env_obs_dim", "dcc_env_reset", "dcc_env_step", "dcc_env_step_features", "dcc_env_obs_write_probe", "dcc_env_rollout", "dcc_env_get_state",
            "dcc_env_set_state", "dcc_env_bytes_per_step", "dcc_env_kernel_choice", "dcc_obs_features", "dcc_obs_features_x",
            "dcc_relu_ln_fwd", "dcc_relu_ln_bwd", "dcc_relu_ln_head_fwd", "dcc_relu_ln_head_bwd", "dcc_mlp_workspace_floats", "dcc_actor_l1_fwd", "dcc_actor_l1_bwd", "dcc_actor_l1_pre_fwd", "dcc_actor_l1_pre_bwd",
            "dcc_ppo_policy_loss",
            "dcc_rollout_sample", "dcc_rollout_record", "dcc_rollout_record_stats", "dcc_ppo_value_loss",
-           "dcc_grad_norm_workspace_floats", "dcc_grad_norm_clip", "dcc_adam_step"]
+           "dcc_grad_norm_workspace_floats", "dcc_grad_norm_clip", "dcc_adam_step",
+           "dcc_delta_ckpt_floats", "dcc_delta_fwd_workspace_floats", "dcc_delta_bwd_workspace_floats", "dcc_delta_fwd", "dcc_delta_bwd",
+           "dcc_delta_step"]
 
 _lib = None
 
@@ -110,6 +125,12 @@ def load_library(path=None):
     L.dcc_grad_norm_workspace_floats.restype = i64
     L.dcc_grad_norm_clip.argtypes = [_vp, i64, f32, _vp, _vp, _vp]
     L.dcc_adam_step.argtypes = [_vp, _vp, _vp, _vp, i64, f32, f32, ctypes.c_double, ctypes.c_double, f32, f32, _vp, _vp]
+    for n in ("dcc_delta_ckpt_floats", "dcc_delta_fwd_workspace_floats", "dcc_delta_bwd_workspace_floats"):
+        getattr(L, n).argtypes = [ctypes.POINTER(DeltaSeq)]
+        getattr(L, n).restype = i64
+    L.dcc_delta_fwd.argtypes = [ctypes.POINTER(DeltaSeq), _vp, _vp]
+    L.dcc_delta_bwd.argtypes = [ctypes.POINTER(DeltaSeq), ctypes.POINTER(DeltaGrad), _vp, _vp]
+    L.dcc_delta_step.argtypes = [ctypes.POINTER(DeltaSeq), _vp]
     if L.dcc_abi_version() != 2:
         raise DccError("libdcc_hip.so ABI version %d != 2" % L.dcc_abi_version())
     _lib = L
@@ -742,3 +763,124 @@ def adam_step(param, grad, exp_avg, exp_avg_sq, step_size, bc2_sqrt, beta1, beta
         _check(load_library().dcc_adam_step(_ptr(param), _ptr(grad), _ptr(exp_avg), _ptr(exp_avg_sq), param.numel(), float(step_size),
                                             float(bc2_sqrt), float(beta1), float(beta2), float(eps), float(weight_decay),
                                             _ptr(clip), _stream()), "dcc_adam_step")
+
+
+# ---- gated delta rule: the memory layer of the recurrent policies (include/dcc_delta.h) -------------------------------
+DELTA_MAX_DIM = 128
+_DELTA_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _delta_seq(what, q, k, v, g, beta, state, masks, scale, lead):
+    """Checks the operands (lead: number of leading axes, 2 = [T, B, ..], 1 = [B, ..]) and fills dcc_delta_seq.
+    -> (struct, operands to keep alive)"""
+    if not (torch.is_tensor(v) and v.is_cuda):
+        raise DccError("%s: v is not on a HIP device (there is no CPU path)" % what)
+    if v.dtype not in _DELTA_DTYPES:
+        raise ValueError("%s: v must be float32, bfloat16 or float16, not %s" % (what, v.dtype))
+    if v.dim() != lead + 2 or not torch.is_tensor(q) or q.dim() != lead + 2:
+        raise ValueError("%s: q and v must have %d axes" % (what, lead + 2))
+    rows, (HK, DK), (H, DV) = tuple(v.shape[:lead]), tuple(q.shape[lead:]), tuple(v.shape[lead:])
+    if not (HK >= 1 and H >= 1 and H % HK == 0 and 1 <= DK <= DELTA_MAX_DIM and 1 <= DV <= DELTA_MAX_DIM):
+        raise ValueError("%s: %d value heads of %d over %d key heads of %d (a multiple; sizes 1..%d)" % (what, H, DV, HK, DK, DELTA_MAX_DIM))
+    want = [("q", q, rows + (HK, DK), v.dtype), ("k", k, rows + (HK, DK), v.dtype), ("v", v, rows + (H, DV), v.dtype),
+            ("g", g, rows + (H,), torch.float32), ("beta", beta, rows + (H,), torch.float32)]
+    if masks is not None:
+        want.append(("masks", masks, rows, torch.float32))
+    if state is not None:
+        want.append(("state", state, (rows[-1], H, DK, DV), torch.float32))
+    for name, t, shape, dt in want:
+        if not torch.is_tensor(t) or tuple(t.shape) != shape or t.dtype != dt or t.device != v.device:
+            raise ValueError("%s: %s must be %s %s on %s" % (what, name, shape, dt, v.device))
+        # (an axis of one element says nothing by its stride)
+        if name in ("q", "k", "v") and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError("%s: the last axis of %s must be contiguous" % (what, name))
+    if state is not None and not state.is_contiguous():
+        raise ValueError("%s: state must be contiguous" % what)
+    s = DeltaSeq()
+    s.T, s.B, s.HK, s.H, s.DK, s.DV = (rows[0] if lead == 2 else 1), rows[-1], HK, H, DK, DV
+    s.dtype, s.scale = _DELTA_DTYPES[v.dtype], float(DK ** -0.5 if scale is None else scale)
+    s.q, s.k, s.v, s.g, s.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
+    s.masks = None if masks is None else masks.data_ptr()
+    s.state0 = None if state is None else state.data_ptr()
+    pad = (0,) if lead == 1 else ()
+    for name, t in (("st_q", q), ("st_k", k), ("st_v", v)):
+        setattr(s, name, (ctypes.c_int64 * 3)(*(pad + tuple(t.stride()[:-1]))))
+    s.st_g, s.st_beta = (ctypes.c_int64 * 3)(*(pad + tuple(g.stride()))), (ctypes.c_int64 * 3)(*(pad + tuple(beta.stride())))
+    if masks is not None:
+        s.st_masks = (ctypes.c_int64 * 2)(*(pad + tuple(masks.stride())))
+    return s
+
+
+def _delta_ws(n, device):
+    return torch.empty(n, dtype=torch.float32, device=device) if n > 0 else None
+
+
+def gated_delta_fwd(q, k, v, g, beta, state=None, masks=None, scale=None, want_ckpt=False):
+    """Gated delta rule over T tokens (include/dcc_delta.h): q, k [T,B,HK,DK], v [T,B,H,DV] (float32 / bfloat16 / float16, last axis
+    contiguous, any other strides), g (log decay) and beta [T,B,H] float32, state [B,H,DK,DV] float32 or None (zero), masks [T,B]
+    float32 or None (0: the state restarts before that token), scale of the output (None: DK ** -0.5).
+    -> o [T,B,H,DV], last state [B,H,DK,DV], what gated_delta_bwd starts from (None unless want_ckpt).  No CPU path."""
+    s = _delta_seq("gated_delta_fwd", q, k, v, g, beta, state, masks, scale, 2)
+    L = load_library()
+    with torch.cuda.device(v.device):
+        o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        last = torch.empty((s.B, s.H, s.DK, s.DV), dtype=torch.float32, device=v.device)
+        ckpt = _delta_ws(max(1, L.dcc_delta_ckpt_floats(ctypes.byref(s))), v.device) if want_ckpt else None
+        ws = _delta_ws(L.dcc_delta_fwd_workspace_floats(ctypes.byref(s)), v.device)
+        s.o, s.state1, s.ckpt = o.data_ptr(), last.data_ptr(), None if ckpt is None else ckpt.data_ptr()
+        _check(L.dcc_delta_fwd(ctypes.byref(s), _ptr(ws), _stream()), "dcc_delta_fwd")
+    return o, last, ckpt
+
+
+def gated_delta_bwd(q, k, v, g, beta, masks, scale, ckpt, dout, dstate=None):
+    """Gradient of gated_delta_fwd: dout [T,B,H,DV] like v, dstate [B,H,DK,DV] float32 or None (zero), ckpt from the forward call.
+    -> dq, dk, dv (like q, k, v), dg, dbeta [T,B,H] float32, d(first state) [B,H,DK,DV] float32."""
+    s = _delta_seq("gated_delta_bwd", q, k, v, g, beta, None, masks, scale, 2)
+    if not torch.is_tensor(dout) or dout.shape != v.shape or dout.dtype != v.dtype or dout.device != v.device:
+        raise ValueError("gated_delta_bwd: dout must be %s %s on %s" % (tuple(v.shape), v.dtype, v.device))
+    if dout.shape[-1] > 1 and dout.stride(-1) != 1:
+        raise ValueError("gated_delta_bwd: the last axis of dout must be contiguous")
+    shape = (s.B, s.H, s.DK, s.DV)
+    if dstate is not None and (tuple(dstate.shape) != shape or dstate.dtype != torch.float32 or dstate.device != v.device or not dstate.is_contiguous()):
+        raise ValueError("gated_delta_bwd: dstate must be contiguous float32 %s on %s" % (shape, v.device))
+    L = load_library()
+    need = max(1, L.dcc_delta_ckpt_floats(ctypes.byref(s)))
+    if not torch.is_tensor(ckpt) or ckpt.dtype != torch.float32 or ckpt.numel() != need or ckpt.device != v.device or not ckpt.is_contiguous():
+        raise ValueError("gated_delta_bwd: ckpt must be the %d floats that gated_delta_fwd(want_ckpt=True) returned for these sizes" % need)
+    with torch.cuda.device(v.device):
+        mk = lambda shape, dt: torch.empty(shape, dtype=dt, device=v.device)
+        dq, dk, dv = mk(q.shape, q.dtype), mk(k.shape, k.dtype), mk(v.shape, v.dtype)
+        dg, dbeta, ds = mk(g.shape, torch.float32), mk(beta.shape, torch.float32), mk(shape, torch.float32)
+        ws = _delta_ws(L.dcc_delta_bwd_workspace_floats(ctypes.byref(s)), v.device)
+        d = DeltaGrad()
+        d.dout, d.st_do, d.ckpt = dout.data_ptr(), (ctypes.c_int64 * 3)(*dout.stride()[:-1]), ckpt.data_ptr()
+        d.dstate1 = None if dstate is None else dstate.data_ptr()
+        d.dq, d.dk, d.dv, d.dg, d.dbeta, d.dstate0 = (t.data_ptr() for t in (dq, dk, dv, dg, dbeta, ds))
+        _check(L.dcc_delta_bwd(ctypes.byref(s), ctypes.byref(d), _ptr(ws), _stream()), "dcc_delta_bwd")
+    return dq, dk, dv, dg, dbeta, ds
+
+
+def gated_delta_step(q, k, v, g, beta, state, masks=None, scale=None, out=None, state_out=None):
+    """One token of the gated delta rule (rollout, serving): q, k [B,HK,DK], v [B,H,DV], g, beta [B,H], state [B,H,DK,DV] float32,
+    masks [B] or None.  out [B,H,DV] and state_out (contiguous; `state` itself: updated in place) are allocated when absent.
+    -> o, new state.  No gradient (the training pass is fused.gated_delta).  No CPU path."""
+    if state is None:
+        raise ValueError("gated_delta_step: a state is needed")
+    s = _delta_seq("gated_delta_step", q, k, v, g, beta, state, masks, scale, 1)
+    for name, t, shape, dt in (("out", out, v.shape, v.dtype), ("state_out", state_out, state.shape, torch.float32)):
+        if t is not None and (not torch.is_tensor(t) or t.shape != shape or t.dtype != dt or t.device != v.device or not t.is_contiguous()):
+            raise ValueError("gated_delta_step: %s must be contiguous %s %s on %s" % (name, tuple(shape), dt, v.device))
+    if state_out is not None and state_out.data_ptr() != state.data_ptr() and _overlap(state, state_out):
+        raise ValueError("gated_delta_step: state_out must be state itself or lie apart from it")
+    with torch.cuda.device(v.device):
+        out = torch.empty(v.shape, dtype=v.dtype, device=v.device) if out is None else out
+        state_out = torch.empty_like(state) if state_out is None else state_out
+        s.o, s.state1 = out.data_ptr(), state_out.data_ptr()
+        _check(load_library().dcc_delta_step(ctypes.byref(s), _stream()), "dcc_delta_step")
+    return out, state_out
+
+
+def _overlap(a, b):
+    """Do two contiguous tensors share memory?"""
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
