@@ -57,6 +57,10 @@ class DeltaGrad(ctypes.Structure):     # include/dcc_delta.h: dcc_delta_grad
                 ("dg", _vp), ("dbeta", _vp), ("dstate0", _vp)]
 
 
+class OrthoMat(ctypes.Structure):      # include/dcc_ortho.h: dcc_ortho_mat
+    _fields_ = [("inp", _vp), ("out", _vp), ("M", ctypes.c_int64), ("N", ctypes.c_int64)]
+
+
 EXPORTS = ["dcc_obs_expand", "dcc_gae_compute", "dcc_returns_compute", "dcc_abi_version", "dcc_last_error", "dcc_env_cfg_default", "dcc_env_create", "dcc_env_destroy",
            "dcc_env_obs_dim", "dcc_env_reset", "dcc_env_step", "dcc_env_step_features", "dcc_env_obs_write_probe", "dcc_env_rollout", "dcc_env_get_state",
            "dcc_env_set_state", "dcc_env_bytes_per_step", "dcc_env_kernel_choice", "dcc_obs_features", "dcc_obs_features_x",
@@ -65,7 +69,7 @@ EXPORTS = ["dcc_obs_expand", "dcc_gae_compute", "dcc_returns_compute", "dcc_abi_
            "dcc_rollout_sample", "dcc_rollout_record", "dcc_rollout_record_stats", "dcc_ppo_value_loss",
            "dcc_grad_norm_workspace_floats", "dcc_grad_norm_clip", "dcc_adam_step",
            "dcc_delta_ckpt_floats", "dcc_delta_fwd_workspace_floats", "dcc_delta_bwd_workspace_floats", "dcc_delta_fwd", "dcc_delta_bwd",
-           "dcc_delta_step"]
+           "dcc_delta_step", "dcc_ortho_workspace_bytes", "dcc_orthogonalize"]
 
 _lib = None
 
@@ -131,6 +135,9 @@ def load_library(path=None):
     L.dcc_delta_fwd.argtypes = [ctypes.POINTER(DeltaSeq), _vp, _vp]
     L.dcc_delta_bwd.argtypes = [ctypes.POINTER(DeltaSeq), ctypes.POINTER(DeltaGrad), _vp, _vp]
     L.dcc_delta_step.argtypes = [ctypes.POINTER(DeltaSeq), _vp]
+    L.dcc_ortho_workspace_bytes.argtypes = [ctypes.POINTER(OrthoMat), i32, i32, i32]
+    L.dcc_ortho_workspace_bytes.restype = i64
+    L.dcc_orthogonalize.argtypes = [ctypes.POINTER(OrthoMat), i32, i32, i32, f32, f32, f32, f32, _vp, _vp]
     if L.dcc_abi_version() != 2:
         raise DccError("libdcc_hip.so ABI version %d != 2" % L.dcc_abi_version())
     _lib = L
@@ -884,3 +891,48 @@ def _overlap(a, b):
     """Do two contiguous tensors share memory?"""
     a0, b0 = a.data_ptr(), b.data_ptr()
     return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+
+
+# ---- orthogonalised updates (include/dcc_ortho.h) ----------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(mats, steps=5, coeffs=NEWTON_SCHULZ, eps=1e-7, out=None):
+    """Newton-Schulz orthogonalisation of every matrix of a list (a tensor [M,N], [..,M,N] or a list of such), as the Muon optimiser
+    takes it: X = G / (|G|_F + eps), transposed when M > N; `steps` times X <- (a I + b A + c A^2) X with A = X X^T, coeffs = (a, b, c).
+    Contiguous float32 / bfloat16 / float16 device tensors of one type; `out`: tensors like them, apart from them (allocated when
+    None).  -> the results, as a tensor or a list like `mats`.  No gradient.  No CPU path."""
+    single = torch.is_tensor(mats)
+    ms = [mats] if single else list(mats)
+    outs = None if out is None else ([out] if single else list(out))
+    if outs is not None and len(outs) != len(ms):
+        raise ValueError("orthogonalize: %d outputs for %d matrices" % (len(outs), len(ms)))
+    if not ms:
+        return []
+    ref = ms[0]
+    for t in ms + (outs or []):
+        if not torch.is_tensor(t) or not t.is_cuda:
+            raise DccError("orthogonalize: tensors on a HIP device (there is no CPU path)")
+        if t.dim() < 2 or t.dtype not in _DELTA_DTYPES or t.dtype != ref.dtype or t.device != ref.device or not t.is_contiguous():
+            raise ValueError("orthogonalize: contiguous [.., M, N] float32 / bfloat16 / float16 tensors of one type on one device")
+    if outs is not None and any(o.shape != t.shape for o, t in zip(outs, ms)):
+        raise ValueError("orthogonalize: outputs must have the shapes of the matrices")
+    if len(coeffs) != 3:
+        raise ValueError("orthogonalize: coeffs = (a, b, c)")
+    L = load_library()
+    dt = _DELTA_DTYPES[ref.dtype]
+    with torch.cuda.device(ref.device):
+        if outs is None:
+            outs = [torch.empty_like(t) for t in ms]
+        flat = []
+        for t, o in zip(ms, outs):
+            M, N = t.shape[-2:]
+            step = M * N * t.element_size()
+            for i in range(t.numel() // (M * N) if M * N else 0):
+                flat.append((t.data_ptr() + i * step, o.data_ptr() + i * step, M, N))
+        arr = (OrthoMat * max(1, len(flat)))(*flat)
+        nbytes = L.dcc_ortho_workspace_bytes(arr, len(flat), dt, int(steps))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=ref.device) if nbytes else None
+        _check(L.dcc_orthogonalize(arr, len(flat), dt, int(steps), float(coeffs[0]), float(coeffs[1]), float(coeffs[2]), float(eps),
+                                   _ptr(ws), _stream()), "dcc_orthogonalize")
+    return outs[0] if single else outs
