@@ -9,9 +9,15 @@ The reference cuts the sequence at the steps where any mask is 0 and runs one mu
 the cut points it copies the masks to the host (`.nonzero().cpu()`: a device synchronisation inside every PPO
 mini-batch).  Multiplying the state by the step's mask before EVERY step is the same arithmetic (the mask is exactly
 1.0 inside a segment) and needs no host round trip, so the update stays asynchronous on the device.
+
+`GatedDeltaLayer` (cfg.recurrent_core: gated_delta) stands in for the GRU with the same call: its state is a matrix per head instead of a
+vector, and a sequence is one launch forward and one backward (include/dcc_delta.h) where the GRU steps through it in Python.
 """
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
+
+from . import fused
 
 
 class RNNLayer(nn.Module):
@@ -41,3 +47,83 @@ class RNNLayer(nn.Module):
                 outs.append(out)
             x = torch.cat(outs, dim=0).reshape(T * B, -1)
         return self.norm(x), h.transpose(0, 1)
+
+
+class GatedDeltaLayer(nn.Module):
+    """`recurrent_N` residual gated-delta layers + LayerNorm, called like RNNLayer with states of heads * head_dim^2 numbers:
+        q, k, v, a, b = W x;   q, k of unit length;   g = -exp(A_log) softplus(a + dt_bias);   beta = sigmoid(b)
+        x <- x + W_o RMSNorm(gated_delta(q, k, v, g, beta))
+    masks restart the state (0: the episode ended before this step)."""
+
+    def __init__(self, inputs_dim, outputs_dim, recurrent_N, use_orthogonal, heads=4, head_dim=32):
+        super().__init__()
+        if inputs_dim != outputs_dim:
+            raise ValueError("GatedDeltaLayer: the residual path needs inputs_dim == outputs_dim")
+        if not (1 <= heads and 1 <= head_dim <= 128):
+            raise ValueError("GatedDeltaLayer: heads >= 1 and 1 <= head_dim <= 128")
+        self._recurrent_N, self.heads, self.head_dim = recurrent_N, heads, head_dim
+        w = heads * head_dim
+        init = nn.init.orthogonal_ if use_orthogonal else nn.init.xavier_uniform_
+        self.qkv, self.gates, self.out = nn.ModuleList(), nn.ModuleList(), nn.ModuleList()
+        self.A_log, self.dt_bias, self.scale = nn.ParameterList(), nn.ParameterList(), nn.ParameterList()
+        for _ in range(recurrent_N):
+            self.qkv.append(nn.Linear(inputs_dim, 3 * w, bias=False))
+            self.gates.append(nn.Linear(inputs_dim, 2 * heads))
+            self.out.append(nn.Linear(w, outputs_dim, bias=False))
+            for lin in (self.qkv[-1], self.gates[-1], self.out[-1]):
+                init(lin.weight)
+            nn.init.constant_(self.gates[-1].bias, 0)
+            # time constants of the heads: decay 1/2 .. 1/64 per step where the gate is at its bias
+            dt = torch.logspace(-1, -6, heads, base=2.0) if heads > 1 else torch.tensor([0.1])
+            self.A_log.append(nn.Parameter(torch.zeros(heads)))
+            self.dt_bias.append(nn.Parameter(torch.log(torch.expm1(dt))))
+            self.scale.append(nn.Parameter(torch.ones(head_dim)))
+        self.norm = nn.LayerNorm(outputs_dim)
+
+    def forward(self, x, hxs, masks):
+        B, H, D = hxs.size(0), self.heads, self.head_dim
+        T = x.size(0) // B
+        m = masks.reshape(T, B).float()
+        states = []
+        for i in range(self._recurrent_N):
+            q, k, v = self.qkv[i](x).view(T, B, 3, H, D).unbind(2)
+            a, b = self.gates[i](x).view(T, B, 2, H).unbind(2)
+            q, k = F.normalize(q, dim=-1), F.normalize(k, dim=-1)
+            g = -torch.exp(self.A_log[i]) * F.softplus(a + self.dt_bias[i])
+            beta = torch.sigmoid(b)
+            S = hxs[:, i].reshape(B, H, D, D)
+            if T == 1 and x.is_cuda and not torch.is_grad_enabled() and not torch.is_autocast_enabled():
+                import dcc_hip
+                o, S = dcc_hip.gated_delta_step(q[0], k[0], v[0], g[0], beta[0], S.contiguous(), m[0])
+            else:
+                o, S = fused.gated_delta(q, k, v, g, beta, S, m)
+            o = o.view(T * B, H, D)
+            o = o * torch.rsqrt(o.square().mean(-1, keepdim=True) + 1e-6) * self.scale[i]
+            x = x + self.out[i](o.view(T * B, H * D))
+            states.append(S.reshape(B, H * D * D))
+        return self.norm(x), torch.stack(states, 1)
+
+
+CORES = ("gru", "gated_delta")
+
+
+def _core(cfg):
+    name = getattr(cfg, "recurrent_core", "gru")
+    if name not in CORES:
+        raise ValueError("recurrent_core: %r is not one of %s" % (name, list(CORES)))
+    return name
+
+
+def make_recurrent(cfg):
+    """The recurrent core that cfg names, between trunk and head."""
+    H = cfg.algo_hidden_size
+    if _core(cfg) == "gru":
+        return RNNLayer(H, H, cfg.recurrent_N, cfg.use_orthogonal)
+    return GatedDeltaLayer(H, H, cfg.recurrent_N, cfg.use_orthogonal, int(getattr(cfg, "delta_heads", 4)), int(getattr(cfg, "delta_head_dim", 32)))
+
+
+def state_size(cfg):
+    """Numbers of recurrent state per row and layer (the last axis of hxs)."""
+    if _core(cfg) == "gru":
+        return cfg.algo_hidden_size
+    return int(getattr(cfg, "delta_heads", 4)) * int(getattr(cfg, "delta_head_dim", 32)) ** 2

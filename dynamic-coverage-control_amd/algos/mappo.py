@@ -25,7 +25,7 @@ import torch
 
 import utils.pytorch_utils as ptu
 from algos.algo_utils import fused
-from algos.algo_utils.optim import FlatAdam
+from algos.algo_utils.optim import make_optimizer
 from algos.algo_utils.structured import invalidate_folded_weights
 from algos.r_actor_critic import R_Actor, R_Critic
 from utils.util import huber_loss, mse_loss, update_linear_schedule
@@ -45,10 +45,10 @@ class MAPPOPolicy:
         self.obs_space, self.share_obs_space, self.act_space = obs_space, cent_obs_space, act_space
         self.actor = R_Actor(cfg, obs_space, act_space, ptu.device)
         self.critic = R_Critic(cfg, cent_obs_space, ptu.device)
-        self.actor_optimizer = FlatAdam(self.actor.parameters(), lr=self.actor_lr, eps=self.opti_eps,
-                                        weight_decay=self.weight_decay)
-        self.critic_optimizer = FlatAdam(self.critic.parameters(), lr=self.critic_lr, eps=self.opti_eps,
-                                         weight_decay=self.weight_decay)
+        self.actor_optimizer = make_optimizer(cfg, self.actor.parameters(), lr=self.actor_lr, eps=self.opti_eps,
+                                              weight_decay=self.weight_decay)
+        self.critic_optimizer = make_optimizer(cfg, self.critic.parameters(), lr=self.critic_lr, eps=self.opti_eps,
+                                               weight_decay=self.weight_decay)
 
     def enable_structured_input(self, layout):
         """Let actor and critic accept compact features (algo_utils/structured.py) in place of observation rows."""

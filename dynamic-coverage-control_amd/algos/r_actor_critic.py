@@ -5,7 +5,7 @@ per network are the only dense contractions of the whole hot path and run on MFM
 hipBLASLt.  Inputs are expected to live on the device already (the rollout never leaves the GPU);
 numpy inputs are still accepted for drop-in use.  The recurrent variants (`use_recurrent_policy`,
 `use_naive_recurrent_policy`: a GRU + LayerNorm between trunk and head, r_actor_critic.py:36-37,52-53,100-101,117-118)
-are built (algo_utils/rnn.py) although the shipped config keeps them off; the CNN / PopArt variants are not
+are built (algo_utils/rnn.py, where a gated delta layer can stand in for the GRU: cfg.recurrent_core) although the shipped config keeps them off; the CNN / PopArt variants are not
 (disabled by mappo.yaml, cfg keys accepted and must be off).
 """
 import torch
@@ -13,7 +13,7 @@ import torch.nn as nn
 
 from algos.algo_utils.act import ACTLayer
 from algos.algo_utils.mlp import MLPBase
-from algos.algo_utils.rnn import RNNLayer
+from algos.algo_utils.rnn import make_recurrent
 from algos.algo_utils import structured
 from algos.algo_utils.util import init
 from utils.util import check
@@ -38,7 +38,7 @@ class R_Actor(nn.Module):
         obs_shape = get_shape_from_obs_space(obs_space)
         _require_mlp(cfg, obs_shape)
         self.base = MLPBase(cfg, obs_shape)
-        self.rnn = RNNLayer(self.hidden_size, self.hidden_size, cfg.recurrent_N, cfg.use_orthogonal) if _recurrent(cfg) else None
+        self.rnn = make_recurrent(cfg) if _recurrent(cfg) else None
         self.act = ACTLayer(action_space, self.hidden_size, cfg.use_orthogonal, cfg.gain)
         self.obs_layout = None    # set by MAPPOPolicy.enable_structured_input
         self.to(device)
@@ -91,7 +91,7 @@ class R_Critic(nn.Module):
         shape = get_shape_from_obs_space(cent_obs_space)
         _require_mlp(cfg, shape)
         self.base = MLPBase(cfg, shape)
-        self.rnn = RNNLayer(self.hidden_size, self.hidden_size, cfg.recurrent_N, cfg.use_orthogonal) if _recurrent(cfg) else None
+        self.rnn = make_recurrent(cfg) if _recurrent(cfg) else None
         init_method = nn.init.orthogonal_ if cfg.use_orthogonal else nn.init.xavier_uniform_
         self.v_out = init(nn.Linear(self.hidden_size, 1), init_method, lambda b: nn.init.constant_(b, 0))
         self.obs_layout = None

@@ -24,6 +24,7 @@ import numpy as np
 import torch
 
 import utils.pytorch_utils as ptu
+from algos.algo_utils.rnn import state_size
 from utils.util import get_shape_from_act_space, get_shape_from_obs_space
 
 
@@ -181,12 +182,12 @@ class SharedReplayBuffer(object):
         self.masks = torch.ones(T + 1, E, N, 1, dtype=torch.float32, device=self.device)
         self.bad_masks = torch.ones_like(self.masks)
         self.active_masks = torch.ones_like(self.masks)
-        # GRU states of the recurrent policy variants (shared_buffer.py:42-45); feed-forward policies (the shipped
+        # states of the recurrent policy variants (shared_buffer.py:42-45); feed-forward policies (the shipped
         # setting) get zero-width placeholders that keep `buffer.rnn_states[t]` indexable
         self.recurrent = bool(cfg.use_recurrent_policy or cfg.use_naive_recurrent_policy)
         if self.recurrent and self.store_state:
             raise ValueError("recurrent policies read observation rows: use structured_input: false, compact_obs: false")
-        self.rnn_states = z(T + 1, E, N, cfg.recurrent_N, cfg.algo_hidden_size if self.recurrent else 0)
+        self.rnn_states = z(T + 1, E, N, cfg.recurrent_N, state_size(cfg) if self.recurrent else 0)
         self.rnn_states_critic = torch.zeros_like(self.rnn_states)
         self.available_actions = None
         self.minibatch_unique_pairs = False     # True: row mini-batches always work on the unique touched (step, env) pairs (tests)

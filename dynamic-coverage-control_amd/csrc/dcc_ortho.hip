@@ -406,6 +406,47 @@ __global__ __launch_bounds__(256) void ortho_djoin_k(const DBatch bt) {
     }
 }
 
+// ---- the element-wise ends of a step: bound by their bytes ---------------------------------------------------------------------
+constexpr int kMaxSegs = 64;
+struct Segs { long long off[kMaxSegs], n[kMaxSegs]; float scale[kMaxSegs]; int first[kMaxSegs + 1]; int count; float keep; };
+
+__global__ __launch_bounds__(256) void muon_momentum_k(const float* __restrict__ g, float* __restrict__ buf, float* __restrict__ dir, long long n,
+                                                       float mu, int nesterov, const float* __restrict__ clip_p) {
+    const float clip = clip_p ? *clip_p : 1.f;
+    const long long n4 = n >> 2;
+    const long long i0 = (long long)blockIdx.x * 256 + threadIdx.x;
+    for (long long i = i0; i < n4 + (n & 3); i += (long long)gridDim.x * 256) {
+        if (i < n4) {
+            f4 x = reinterpret_cast<const f4*>(g)[i], m = reinterpret_cast<f4*>(buf)[i];
+            x *= clip;
+            m = mu * m + x;
+            reinterpret_cast<f4*>(buf)[i] = m;
+            reinterpret_cast<f4*>(dir)[i] = nesterov ? x + mu * m : m;
+        } else {
+            const long long e = (n4 << 2) + (i - n4);
+            const float x = g[e] * clip, m = mu * buf[e] + x;
+            buf[e] = m;
+            dir[e] = nesterov ? x + mu * m : m;
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void muon_apply_k(float* __restrict__ p, const float* __restrict__ dir, const Segs s) {
+    int q = 0;
+    while (q + 1 < s.count && (int)blockIdx.x >= s.first[q + 1]) ++q;
+    const long long lo = s.off[q] + (long long)(blockIdx.x - s.first[q]) * 4096, end = s.off[q] + s.n[q];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const long long i = lo + j * 1024 + 4 * threadIdx.x;
+        if (i + 3 < end) {
+            const f4 v = s.keep * *reinterpret_cast<const f4*>(p + i) - s.scale[q] * *reinterpret_cast<const f4*>(dir + i);
+            *reinterpret_cast<f4*>(p + i) = v;
+        } else {
+            for (long long e = i; e < end && e < i + 4; ++e) p[e] = s.keep * p[e] - s.scale[q] * dir[e];
+        }
+    }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kAlign = 256;
 int64_t up(int64_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
@@ -667,6 +708,42 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
     return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string("dcc_orthogonalize: ") + hipGetErrorString(e));
 } catch (...) {
     return dcc_fail(kEINVAL, "dcc_orthogonalize: out of host memory");
+}
+
+DCC_API int dcc_muon_momentum(const float* grad, float* buf, float* dir, int64_t n, float momentum, int32_t nesterov, const float* clip,
+                              void* stream) {
+    if (!grad || !buf || !dir || n < 1) return dcc_fail(kEINVAL, "dcc_muon_momentum: null pointer or n < 1");
+    if ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(buf) | reinterpret_cast<uintptr_t>(dir)) & 15)
+        return dcc_fail(kEINVAL, "dcc_muon_momentum: arrays must be 16-byte aligned");
+    const int64_t nb = std::min<int64_t>(((n >> 2) + 3 + 255) / 256, 2048);
+    hipLaunchKernelGGL(muon_momentum_k, dim3((unsigned)nb), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), grad, buf, dir, (long long)n, momentum,
+                       nesterov, clip);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string("dcc_muon_momentum: ") + hipGetErrorString(e));
+}
+
+DCC_API int dcc_muon_apply(float* param, const float* dir, const dcc_muon_seg* segs, int32_t count, float keep, void* stream) {
+    if (count < 0 || !param || !dir || (count > 0 && !segs)) return dcc_fail(kEINVAL, "dcc_muon_apply: null pointer or negative count");
+    if ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(dir)) & 15) return dcc_fail(kEINVAL, "dcc_muon_apply: arrays must be 16-byte aligned");
+    for (int i = 0; i < count; ++i)
+        if (segs[i].offset < 0 || segs[i].offset % 4 || segs[i].numel < 0 || segs[i].numel > (1ll << 40))
+            return dcc_fail(kEINVAL, "dcc_muon_apply: a range must start at a multiple of 4 and hold 0..2^40 elements");
+    for (int from = 0; from < count; from += kMaxSegs) {
+        Segs s;
+        s.count = 0;
+        s.keep = keep;
+        int64_t first = 0;
+        for (int i = from; i < count && i < from + kMaxSegs; ++i) {
+            if (segs[i].numel == 0) continue;
+            s.off[s.count] = segs[i].offset; s.n[s.count] = segs[i].numel; s.scale[s.count] = segs[i].scale; s.first[s.count] = (int)first;
+            first += (segs[i].numel + 4095) / 4096;
+            ++s.count;
+        }
+        if (first > 2147483647) return dcc_fail(kEINVAL, "dcc_muon_apply: more than 2^43 elements in one list");
+        if (s.count) hipLaunchKernelGGL(muon_apply_k, dim3((unsigned)first), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), param, dir, s);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string("dcc_muon_apply: ") + hipGetErrorString(e));
 }
 
 }  // extern "C"

@@ -61,6 +61,10 @@ class OrthoMat(ctypes.Structure):      # include/dcc_ortho.h: dcc_ortho_mat
     _fields_ = [("inp", _vp), ("out", _vp), ("M", ctypes.c_int64), ("N", ctypes.c_int64)]
 
 
+class MuonSeg(ctypes.Structure):       # include/dcc_ortho.h: dcc_muon_seg
+    _fields_ = [("offset", ctypes.c_int64), ("numel", ctypes.c_int64), ("scale", ctypes.c_float)]
+
+
 EXPORTS = ["dcc_obs_expand", "dcc_gae_compute", "dcc_returns_compute", "dcc_abi_version", "dcc_last_error", "dcc_env_cfg_default", "dcc_env_create", "dcc_env_destroy",
            "dcc_env_obs_dim", "dcc_env_reset", "dcc_env_step", "dcc_env_step_features", "dcc_env_obs_write_probe", "dcc_env_rollout", "dcc_env_get_state",
            "dcc_env_set_state", "dcc_env_bytes_per_step", "dcc_env_kernel_choice", "dcc_obs_features", "dcc_obs_features_x",
@@ -69,7 +73,7 @@ EXPORTS = ["dcc_obs_expand", "dcc_gae_compute", "dcc_returns_compute", "dcc_abi_
            "dcc_rollout_sample", "dcc_rollout_record", "dcc_rollout_record_stats", "dcc_ppo_value_loss",
            "dcc_grad_norm_workspace_floats", "dcc_grad_norm_clip", "dcc_adam_step",
            "dcc_delta_ckpt_floats", "dcc_delta_fwd_workspace_floats", "dcc_delta_bwd_workspace_floats", "dcc_delta_fwd", "dcc_delta_bwd",
-           "dcc_delta_step", "dcc_ortho_workspace_bytes", "dcc_orthogonalize"]
+           "dcc_delta_step", "dcc_ortho_workspace_bytes", "dcc_orthogonalize", "dcc_muon_momentum", "dcc_muon_apply"]
 
 _lib = None
 
@@ -138,6 +142,8 @@ def load_library(path=None):
     L.dcc_ortho_workspace_bytes.argtypes = [ctypes.POINTER(OrthoMat), i32, i32, i32]
     L.dcc_ortho_workspace_bytes.restype = i64
     L.dcc_orthogonalize.argtypes = [ctypes.POINTER(OrthoMat), i32, i32, i32, f32, f32, f32, f32, _vp, _vp]
+    L.dcc_muon_momentum.argtypes = [_vp, _vp, _vp, i64, f32, i32, _vp, _vp]
+    L.dcc_muon_apply.argtypes = [_vp, _vp, ctypes.POINTER(MuonSeg), i32, f32, _vp]
     if L.dcc_abi_version() != 2:
         raise DccError("libdcc_hip.so ABI version %d != 2" % L.dcc_abi_version())
     _lib = L
@@ -936,3 +942,29 @@ def orthogonalize(mats, steps=5, coeffs=NEWTON_SCHULZ, eps=1e-7, out=None):
         _check(L.dcc_orthogonalize(arr, len(flat), dt, int(steps), float(coeffs[0]), float(coeffs[1]), float(coeffs[2]), float(eps),
                                    _ptr(ws), _stream()), "dcc_orthogonalize")
     return outs[0] if single else outs
+
+
+def muon_momentum(grad, buf, direction, momentum, nesterov=True, clip=None):
+    """buf = momentum * buf + clip * grad; direction = clip * grad + momentum * buf (nesterov) or buf, on flat float32 arrays."""
+    for t, nm in ((grad, "grad"), (buf, "buf"), (direction, "direction")):
+        _f32c(t, nm)
+        if t.numel() != grad.numel() or t.device != grad.device:
+            raise ValueError("muon_momentum: %s has %d elements on %s, grad %d on %s" % (nm, t.numel(), t.device, grad.numel(), grad.device))
+    with torch.cuda.device(grad.device):
+        _check(load_library().dcc_muon_momentum(_ptr(grad), _ptr(buf), _ptr(direction), grad.numel(), float(momentum), int(bool(nesterov)),
+                                                _ptr(clip), _stream()), "dcc_muon_momentum")
+
+
+def muon_apply(param, direction, segs, keep=1.0):
+    """param = keep * param - scale * direction on the ranges segs = [(offset, numel, scale)] of flat float32 arrays."""
+    _f32c(param, "param"); _f32c(direction, "direction")
+    if direction.numel() != param.numel() or direction.device != param.device:
+        raise ValueError("muon_apply: direction must have param's size and device")
+    arr = (MuonSeg * max(1, len(segs)))(*segs)
+    end = 0
+    for s in sorted(segs):
+        if s[0] < end or s[0] + s[1] > param.numel():
+            raise ValueError("muon_apply: ranges must lie apart from each other and within %d elements" % param.numel())
+        end = s[0] + s[1]
+    with torch.cuda.device(param.device):
+        _check(load_library().dcc_muon_apply(_ptr(param), _ptr(direction), arr, len(segs), float(keep), _stream()), "dcc_muon_apply")

@@ -501,7 +501,8 @@ class Learner:
         cov_max = torch.zeros(E, device=ptu.device)
         rnn = masks = None
         if self.recurrent:
-            rnn = torch.zeros(E * N, self.cfg.recurrent_N, self.cfg.algo_hidden_size, device=ptu.device)
+            from algos.algo_utils.rnn import state_size
+            rnn = torch.zeros(E * N, self.cfg.recurrent_N, state_size(self.cfg), device=ptu.device)
             masks = torch.ones(E * N, 1, device=ptu.device)
         for t in range(T):
             if deterministic or noise_scale == 1.0:

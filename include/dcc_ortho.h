@@ -49,6 +49,18 @@ DCC_API int64_t dcc_ortho_workspace_bytes(const dcc_ortho_mat* mats, int32_t cou
 DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t dtype, int32_t steps, float a, float b, float c,
                               float eps, void* workspace, void* stream);
 
+/* The two element-wise ends of a Muon step on flat float32 arrays (16-byte aligned):
+ *   dcc_muon_momentum   g = clip * grad;  buf = momentum * buf + g;  dir = nesterov ? g + momentum * buf : buf
+ *                       (clip: device pointer to the scale of the gradient, NULL = 1; dcc_grad_norm_clip leaves it)
+ *   dcc_muon_apply      param = keep * param - segs[i].scale * dir on every range of the list (ranges must not overlap) */
+typedef struct {
+    int64_t offset, numel;       /* in elements; the offset a multiple of 4 */
+    float scale;
+} dcc_muon_seg;
+DCC_API int dcc_muon_momentum(const float* grad, float* buf, float* dir, int64_t n, float momentum, int32_t nesterov, const float* clip,
+                              void* stream);
+DCC_API int dcc_muon_apply(float* param, const float* dir, const dcc_muon_seg* segs, int32_t count, float keep, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
