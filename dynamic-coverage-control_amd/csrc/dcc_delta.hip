@@ -29,10 +29,10 @@ namespace {
 
 constexpr int kEINVAL = -1, kEHIP = -2;
 constexpr int kC = 16;                  // tokens per chunk
-constexpr int kMaxWaves = 4;
 constexpr float kDead = -103.98f;       // exp() below this is 0 in float32: a restart
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 
 template <typename E> struct Elem;
 template <> struct Elem<float> {
@@ -94,50 +94,79 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
-// `rows` rows of `dim` elements (row i: base + i * stride; rows >= valid and columns >= dim are zero) into LDS rows of `pitch` floats
-template <typename E>
-__device__ __forceinline__ void load_rows(float* dst, int pitch, const void* base, long long stride, int rows, int valid, int dim, int dimp,
-                                          int vec, float mul) {
-    const E* src = reinterpret_cast<const E*>(base);
-    const int c4 = dimp >> 2;
-    for (int e = threadIdx.x; e < rows * c4; e += blockDim.x) {
-        const int i = e / c4, c = (e - i * c4) << 2;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < valid) {
-            const E* p = src + (long long)i * stride + c;
-            if (vec && c + 3 < dim) {
-                x = Elem<E>::get4(*reinterpret_cast<const typename Elem<E>::vec*>(p));
+// A state [DK, DV] through a buffer descriptor: 32-bit offsets, rows and columns outside it read 0 and write nothing.
+constexpr unsigned kOutside = 0x40000000u;      // byte offset of lanes without a column
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t state_rsrc(const float* base, const Seq& p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, p.DK * p.DV * 4, 0x00027000);
+}
+__device__ __forceinline__ float state_load(__amdgpu_buffer_rsrc_t rs, unsigned off) {
+    return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+}
+__device__ __forceinline__ void state_store(float v, __amdgpu_buffer_rsrc_t rs, unsigned off) {
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rs, off, 0, 0);
+}
+
+// ROWS rows of DIMP columns from global memory (row i: base + i * stride; rows >= valid and columns >= dim are zero; valid >= 1) to LDS
+// rows of `pitch` floats, in two halves: all loads are under way before the first is waited for, and other work fits in between.
+// Out-of-range places read a valid one instead and are cleared afterwards: no branches.  VEC: dim, strides and base are multiples of four.
+template <typename E, int ROWS, int DIMP, int NTHR, bool VEC>
+struct RowTile {
+    static constexpr int C4 = DIMP / 4, N = (ROWS * C4 + NTHR - 1) / NTHR;
+    typename Elem<E>::vec raw[N];
+    __device__ __forceinline__ void issue(const E* base, long long stride, int valid, int dim) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int e = threadIdx.x + n * NTHR, i = e / C4, c = (e % C4) * 4;
+            const E* row = base + (long long)(i < valid ? i : valid - 1) * stride;
+            if constexpr (VEC) {
+                raw[n] = *reinterpret_cast<const typename Elem<E>::vec*>(row + (c < dim ? c : 0));
             } else {
-                if (c < dim) x.x = Elem<E>::get(p[0]);
-                if (c + 1 < dim) x.y = Elem<E>::get(p[1]);
-                if (c + 2 < dim) x.z = Elem<E>::get(p[2]);
-                if (c + 3 < dim) x.w = Elem<E>::get(p[3]);
+                E* x = reinterpret_cast<E*>(&raw[n]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = row[c + j < dim ? c + j : 0];
             }
         }
-        f4 y = {x.x * mul, x.y * mul, x.z * mul, x.w * mul};
-        *reinterpret_cast<f4*>(dst + i * pitch + c) = y;
     }
-}
+    __device__ __forceinline__ void commit(float* dst, int pitch, int valid, int dim, float mul) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int e = threadIdx.x + n * NTHR, i = e / C4, c = (e % C4) * 4;
+            if (N * NTHR == ROWS * C4 || e < ROWS * C4) {
+                const float4 x = Elem<E>::get4(raw[n]);
+                f4 y = {x.x * mul, x.y * mul, x.z * mul, x.w * mul};
+                const bool in = i < valid;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = in && c + (VEC ? 0 : j) < dim ? y[j] : 0.f;
+                *reinterpret_cast<f4*>(dst + i * pitch + c) = y;
+            }
+        }
+    }
+};
 
 constexpr int kSP = 20;                         // pitch of the 16x16 tiles in LDS (rows 16-byte aligned)
 struct ChunkVec { float beta[kC], gam[kC], toend[kC], seg[kC], gend; float pad[3]; };     // per chunk: gates as the products use them
 
+// The gates of one token as they come from memory
+struct Gate { float g, beta; int cut; };
+__device__ __forceinline__ Gate load_gate(const Seq& p, long long b, int h, long long t) {
+    const bool in = t < p.T;
+    t = in ? t : p.T - 1;
+    Gate x;
+    x.g = p.g[t * p.sg[0] + b * p.sg[1] + h * p.sg[2]];
+    x.beta = p.beta[t * p.sb[0] + b * p.sb[1] + h * p.sb[2]];
+    const float m = p.masks ? p.masks[t * p.sm[0] + b * p.sm[1]] : 1.f;
+    x.cut = in && (m == 0.f || x.g < kDead);
+    x.g = x.cut || !in ? 0.f : x.g;
+    x.beta = in ? x.beta : 0.f;
+    return x;
+}
+
 // Decays of one chunk, by one wave: lane l works on token l % 16 (the four groups repeat each other).  Running sums in double: the
 // difference of two float sums would carry the error of the larger one into every D_ij.  Returns this lane's running sum and segment.
-__device__ __forceinline__ void chunk_gates(const Seq& p, long long b, int h, long long t0, int lane, double& run, int& seg, ChunkVec* cv) {
+__device__ __forceinline__ void chunk_gates(const Gate& x, int lane, double& run, int& seg, ChunkVec* cv) {
     const int i = lane & 15;
-    const long long t = t0 + i;
-    float g = 0.f, be = 0.f;
-    int cut = 0;
-    if (t < p.T) {
-        g = p.g[t * p.sg[0] + b * p.sg[1] + h * p.sg[2]];
-        be = p.beta[t * p.sb[0] + b * p.sb[1] + h * p.sb[2]];
-        if (p.masks) cut = p.masks[t * p.sm[0] + b * p.sm[1]] == 0.f;
-        if (g < kDead) cut = 1;
-        if (cut) g = 0.f;
-    }
-    double s = (double)g;
-    int c = cut;
+    double s = (double)x.g;
+    int c = x.cut;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) {
         const double su = __shfl_up(s, o, 16);
@@ -149,11 +178,12 @@ __device__ __forceinline__ void chunk_gates(const Seq& p, long long b, int h, lo
     const double send = __shfl(s, 15, 16);
     const int cend = __shfl(c, 15, 16);
     if (lane < 16) {
-        cv->beta[i] = be;
-        cv->gam[i] = c == 0 ? expf((float)s) : 0.f;
+        const float e = c == 0 ? expf((float)s) : 0.f;
+        cv->beta[i] = x.beta;
+        cv->gam[i] = e;
         cv->toend[i] = c == cend ? expf((float)(send - s)) : 0.f;
-        cv->seg[i] = cut ? -1.f - c : (float)c;         // sign: a restart at this token
-        if (i == 15) cv->gend = c == 0 ? expf((float)s) : 0.f;
+        cv->seg[i] = x.cut ? -1.f - c : (float)c;         // sign: a restart at this token
+        if (i == 15) cv->gend = e;
     }
 }
 
@@ -171,8 +201,9 @@ __device__ __forceinline__ f4 chunk_decay(double run, int seg, int lane) {
     return d;
 }
 
-// (I + L)^-1 in place, L strictly lower triangular in `t` [16][kSP]; one wave, lane l solves column l % 16 by forward substitution
-__device__ __forceinline__ void unit_lower_inverse(float* t, int lane) {
+// (I + L)^-1 -> `t` [16][kSP]; this lane holds L[4*(lane/16) + r][lane % 16], strictly lower triangular.  Lane l solves column l % 16 by
+// forward substitution; the entries of L come by lane reads, so nothing waits on memory.
+__device__ __forceinline__ void unit_lower_inverse(const f4& L, float* t, int lane) {
     const int c = lane & 15;
     float x[kC];
 #pragma unroll
@@ -180,105 +211,141 @@ __device__ __forceinline__ void unit_lower_inverse(float* t, int lane) {
         float a = i == c ? 1.f : 0.f;
 #pragma unroll
         for (int j = 0; j < kC; ++j)
-            if (j < i) a -= t[i * kSP + j] * x[j];
+            if (j < i) a -= __int_as_float(__builtin_amdgcn_readlane(__float_as_int(L[i & 3]), 16 * (i >> 2) + j)) * x[j];
         x[i] = a;
+        __builtin_amdgcn_sched_barrier(0);      // or all 120 lane reads are taken first, and spilled
     }
-    wave_sync();        // every lane has read t
     if (lane < 16) {
 #pragma unroll
         for (int i = 0; i < kC; ++i) t[i * kSP + c] = x[i];
     }
 }
 
+// K K^T and Q K^T of one chunk from its LDS rows
+template <int DKT>
+__device__ __forceinline__ void chunk_products(const float* kr, const float* qr, f4& kk, f4& qk) {
+    f4 k0 = zero4(), k1 = zero4(), q0 = zero4(), q1 = zero4();
+#pragma unroll
+    for (int t = 0; t < DKT; ++t) {
+        const f4 a = lds4(kr + 16 * t), e = lds4(qr + 16 * t);
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+            k0 = mfma(a[r], a[r], k0);
+            q0 = mfma(e[r], a[r], q0);
+            k1 = mfma(a[r + 1], a[r + 1], k1);
+            q1 = mfma(e[r + 1], a[r + 1], q1);
+        }
+    }
+    kk = k0 + k1;
+    qk = q0 + q1;
+}
+
 // ---- forward -------------------------------------------------------------------------------------------------------------------
-// One workgroup per (row, head) and up to kMaxWaves tiles of 16 value columns; each wave keeps its [DK, 16] slice of the state in
-// registers and walks the chunks.  Blocks of BT chunks are staged in LDS: the waves first split the state-free part (K K^T, Q K^T, gates,
-// inverse) of the BT chunks among them, then every wave runs the BT chunks on its own columns without a barrier.
-template <typename E, int DKT, int BT>
-__global__ __launch_bounds__(256) void delta_fwd_k(const Seq p) {
-    constexpr int DKP = DKT * 16, KP = DKP + 4;
+// One workgroup per (row, head) and NW tiles of 16 value columns; each wave keeps its [DK, 16] slice of the state in registers and
+// walks the chunks.  Blocks of BT chunks are staged in LDS: the waves first split the state-free part (K K^T, Q K^T, gates, inverse) of
+// the BT chunks among them, then every wave runs the BT chunks on its own columns without a barrier, while the next block is loading.
+template <typename E, int DKT, int BT, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4 ? 2 : 3))) void delta_fwd_k(const Seq p) {
+    constexpr int DKP = DKT * 16, KP = DKP + 4, CPW = (BT + NW - 1) / NW;
     extern __shared__ float sh[];
     float* Ks = sh;
     float* Qs = Ks + BT * kC * KP;
     float* Ti = Qs + BT * kC * KP;              // [BT][16][kSP] inverse
     float* Am = Ti + BT * kC * kSP;             // [BT][16][kSP] (Q K^T) . D
     ChunkVec* cvs = reinterpret_cast<ChunkVec*>(Am + BT * kC * kSP);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = lane & 15, g4 = (lane >> 4) << 2;
     const long long bh = blockIdx.x, b = bh / p.H;
     const int h = (int)(bh - b * p.H), hk = h / p.rep;
-    const int tile = blockIdx.y * nw + wave, col = tile * 16 + li;
+    const int tile = blockIdx.y * NW + wave, col = tile * 16 + li;
     const bool live = tile * 16 < p.DV, mine = col < p.DV;
     const E* q = reinterpret_cast<const E*>(p.q) + b * p.sq[1] + hk * p.sq[2];
     const E* k = reinterpret_cast<const E*>(p.k) + b * p.sk[1] + hk * p.sk[2];
-    const E* v = reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2];
-    E* o = reinterpret_cast<E*>(p.o) + (b * p.H + h) * (long long)p.DV;
+    const E* v = reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2] + (mine ? col : 0);
+    E* o = reinterpret_cast<E*>(p.o) + bh * (long long)p.DV + col;
     const long long so = p.B * p.H * (long long)p.DV, sst = (long long)p.DK * p.DV;
+    const unsigned srow = 4u * p.DV, soff = mine ? 4u * (g4 * p.DV + col) : kOutside;   // state element (16 t + 4 g + r, col): soff + (16 t + r) * srow
 
     f4 S[DKT];
 #pragma unroll
     for (int t = 0; t < DKT; ++t) S[t] = zero4();
-    if (p.state0 && mine) {
+    if (p.state0) {
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.state0 + bh * sst, p);
 #pragma unroll
         for (int t = 0; t < DKT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = 16 * t + g4 + r;
-                if (d < p.DK) S[t][r] = p.state0[bh * sst + (long long)d * p.DV + col];
-            }
+            for (int r = 0; r < 4; ++r) S[t][r] = state_load(rs, soff + (16 * t + r) * srow);
     }
+    auto store_state = [&](float* base) {
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(base, p);
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) state_store(S[t][r], rs, soff + (16 * t + r) * srow);
+    };
+    RowTile<E, BT * kC, DKP, 64 * NW, VEC> rk, rq;
+    Gate gate[CPW];
+    E vnext[4];
+    auto valid_of = [&](int c0) {
+        const long long left = p.T - (long long)c0 * kC;
+        return left < BT * kC ? (int)left : BT * kC;
+    };
+    auto fetch = [&](int c0) {
+        const long long t0 = (long long)c0 * kC;
+        const int valid = valid_of(c0);
+        rk.issue(k + t0 * p.sk[0], p.sk[0], valid, p.DK);
+        rq.issue(q + t0 * p.sq[0], p.sq[0], valid, p.DK);
+#pragma unroll
+        for (int n = 0; n < CPW; ++n) gate[n] = load_gate(p, b, h, t0 + (wave + n * NW) * kC + li);
+    };
+    auto fetch_v = [&](long long t0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const long long t = t0 + g4 + r;
+            vnext[r] = v[(t < p.T ? t : p.T - 1) * p.sv[0]];
+        }
+    };
+    if (p.nchunk > 0) { fetch(0); fetch_v(0); }
     for (int c0 = 0; c0 < p.nchunk; c0 += BT) {
         const long long t0 = (long long)c0 * kC;
-        const long long left = p.T - t0;
-        const int valid = left < BT * kC ? (int)left : BT * kC;
-        const int nc = (valid + kC - 1) / kC;
+        const int nc = p.nchunk - c0 < BT ? p.nchunk - c0 : BT, valid = valid_of(c0);
         __syncthreads();
-        load_rows<E>(Ks, KP, k + t0 * p.sk[0], p.sk[0], nc * kC, valid, p.DK, DKP, p.vec, 1.f);
-        load_rows<E>(Qs, KP, q + t0 * p.sq[0], p.sq[0], nc * kC, valid, p.DK, DKP, p.vec, 1.f);
+        rk.commit(Ks, KP, valid, p.DK, 1.f);
+        rq.commit(Qs, KP, valid, p.DK, 1.f);
+        Gate now[CPW];
+#pragma unroll
+        for (int n = 0; n < CPW; ++n) now[n] = gate[n];
         __syncthreads();
-        for (int c = wave; c < nc; c += nw) {
+        if (c0 + BT < p.nchunk) fetch(c0 + BT);
+#pragma unroll
+        for (int n = 0; n < CPW; ++n) {
+            const int c = wave + n * NW;
+            if (c >= nc) continue;
             double run; int seg;
-            chunk_gates(p, b, h, t0 + c * kC, lane, run, seg, cvs + c);
+            chunk_gates(now[n], lane, run, seg, cvs + c);
             const f4 D = chunk_decay(run, seg, lane);
-            f4 kk = zero4(), qk = zero4();
-            const float* kr = Ks + (c * kC + li) * KP + g4;
-            const float* qr = Qs + (c * kC + li) * KP + g4;
-#pragma unroll
-            for (int t = 0; t < DKT; ++t) {
-                const f4 a = lds4(kr + 16 * t), e = lds4(qr + 16 * t);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) { kk = mfma(a[r], a[r], kk); qk = mfma(e[r], a[r], qk); }
-            }
+            f4 kk, qk, L;
+            chunk_products<DKT>(Ks + (c * kC + li) * KP + g4, Qs + (c * kC + li) * KP + g4, kk, qk);
             wave_sync();
+            const f4 be = lds4(cvs[c].beta + g4);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = g4 + r;
-                Ti[(c * kC + i) * kSP + li] = i > li ? cvs[c].beta[i] * D[r] * kk[r] : 0.f;
+                L[r] = i > li ? be[r] * D[r] * kk[r] : 0.f;
                 Am[(c * kC + i) * kSP + li] = i >= li ? D[r] * qk[r] : 0.f;
             }
-            wave_sync();
-            unit_lower_inverse(Ti + c * kC * kSP, lane);
+            unit_lower_inverse(L, Ti + c * kC * kSP, lane);
         }
         __syncthreads();
         if (live) {
+#pragma unroll 1
             for (int c = 0; c < nc; ++c) {
                 const long long tc = t0 + c * kC;
                 f4 vv;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const long long t = tc + g4 + r;
-                    vv[r] = (mine && t < p.T) ? Elem<E>::get(v[t * p.sv[0] + col]) : 0.f;
-                }
-                if (p.ckpt && mine) {
-                    float* ck = p.ckpt + (bh * (p.nchunk + 1) + c0 + c) * sst + col;
-#pragma unroll
-                    for (int t = 0; t < DKT; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int d = 16 * t + g4 + r;
-                            if (d < p.DK) ck[(long long)d * p.DV] = S[t][r];
-                        }
-                }
+                for (int r = 0; r < 4; ++r) vv[r] = mine && tc + g4 + r < p.T ? Elem<E>::get(vnext[r]) : 0.f;
+                if (c0 + c + 1 < p.nchunk) fetch_v(tc + kC);
+                if (p.ckpt) store_state(p.ckpt + (bh * (p.nchunk + 1) + c0 + c) * sst);
                 const float* kr = Ks + (c * kC + li) * KP + g4;
                 const float* qr = Qs + (c * kC + li) * KP + g4;
                 f4 ks = zero4(), qs = zero4();
@@ -300,73 +367,68 @@ __global__ __launch_bounds__(256) void delta_fwd_k(const Seq p) {
                 f4 u = zero4();
 #pragma unroll
                 for (int r = 0; r < 4; ++r) u = mfma(ti[r], rhs[r], u);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) out = mfma(am[r], u[r], out);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const long long t = tc + g4 + r;
-                    if (mine && t < p.T) o[t * so + col] = Elem<E>::put(out[r] * p.scale);
-                }
                 const float ge = cv.gend;
                 const float* kc = Ks + (c * kC + g4) * KP + li;
                 f4 ud;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) ud[r] = u[r] * de[r];
 #pragma unroll
-                for (int t = 0; t < DKT; ++t) {
+                for (int r = 0; r < 4; ++r) out = mfma(am[r], u[r], out);
+#pragma unroll
+                for (int t = 0; t < DKT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) S[t][r] = ge == 0.f ? 0.f : ge * S[t][r];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) S[t] = mfma(kc[r * KP + 16 * t], ud[r], S[t]);
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int t = 0; t < DKT; ++t) S[t] = mfma(kc[r * KP + 16 * t], ud[r], S[t]);
+                E* oc = o + (tc + g4) * so;
+                if (mine && tc + kC <= p.T) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) oc[r * so] = Elem<E>::put(out[r] * p.scale);
+                } else if (mine) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (tc + g4 + r < p.T) oc[r * so] = Elem<E>::put(out[r] * p.scale);
                 }
             }
         }
     }
-    if (live && mine) {
-        float* outs[2] = {p.state_out ? p.state_out + bh * sst + col : nullptr,
-                          p.ckpt ? p.ckpt + (bh * (p.nchunk + 1) + p.nchunk) * sst + col : nullptr};
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-            if (outs[w]) {
-#pragma unroll
-                for (int t = 0; t < DKT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int d = 16 * t + g4 + r;
-                        if (d < p.DK) outs[w][(long long)d * p.DV] = S[t][r];
-                    }
-            }
+    if (live) {
+        if (p.state_out) store_state(p.state_out + bh * sst);
+        if (p.ckpt) store_state(p.ckpt + (bh * (p.nchunk + 1) + p.nchunk) * sst);
     }
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------------------
-// One workgroup per (row, head), chunks from the last to the first, d(state) in registers (wave w: value tiles w, w + 4).  Per chunk:
+// One workgroup per (row, head), chunks from the last to the first, d(state) in registers (wave w: value tiles w, w + NW).  Per chunk:
 //   dU = A^T do + D_C K dS,  Y = (I + beta N)^-T dU,  X = beta Y,  dV = X,  dbeta = Y . (V - gam K S0 - N U)      (by value columns)
 //   dS <- gam_C dS + Q^T (gam do) - K^T (gam X)                                                                    (by value columns)
 //   dQ = gam do S0^T + (do U^T . D) K                                                                              (by key columns)
 //   dK = (do U^T . D)^T Q + D_C U dS^T - gam X S0^T + (Z + Z^T) K,   Z = -(X U^T . D), strictly lower              (by key columns)
 //   dg_t = sum over s >= t of the same segment (q_s.dq_s - v_s.dv_s), + <dS_C, S_C> if no restart follows in the chunk
 // (the last line sums <dS', S'> from the chunk's end, where it is taken whole: no running sum crosses a chunk).  S0 comes from the
-// checkpoints of the forward pass; U, X, dS pass through LDS where the contraction changes from key to value columns.
-template <typename E, int DKT, int DVT>
-__global__ __launch_bounds__(256) void delta_bwd_k(const Seq p) {
+// checkpoints of the forward pass; U, X, dS pass through LDS where the contraction changes from key to value columns.  Between the two
+// halves, waves 0 and 1 form do U^T and X U^T while waves 2 and 3 prepare the state-free part of the chunk that comes next; its rows were
+// loaded one chunk ahead.  Three barriers per chunk.
+struct ChunkTiles { float Ti[kC * kSP], Am[kC * kSP], Nm[kC * kSP], Dm[kC * kSP]; ChunkVec cv; };
+
+template <typename E, int DKT, int DVT, int NW, bool VEC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void delta_bwd_k(const Seq p) {
     constexpr int DKP = DKT * 16, KP = DKP + 4, DVP = DVT * 16, VP = DVP + 4;
-    constexpr int TPW = (DVT + kMaxWaves - 1) / kMaxWaves, KPW = (DKT + kMaxWaves - 1) / kMaxWaves;
+    constexpr int TPW = (DVT + NW - 1) / NW, KPW = (DKT + NW - 1) / NW;
     extern __shared__ float sh[];
-    float* Ks = sh;
-    float* Qs = Ks + kC * KP;
-    float* Us = Qs + kC * KP;
+    float* Kb = sh;                             // [2][16][KP], by parity of the chunk
+    float* Qb = Kb + 2 * kC * KP;
+    float* Ob = Qb + 2 * kC * KP;               // [2][16][VP]: scale * do
+    float* Us = Ob + 2 * kC * VP;
     float* Xs = Us + kC * VP;
-    float* Os = Xs + kC * VP;                   // scale * do
-    float* dSs = Os + kC * VP;                  // [DKP][VP]
-    float* Ti = dSs + DKP * VP;
-    float* Am = Ti + kC * kSP;
-    float* Nm = Am + kC * kSP;
-    float* Dm = Nm + kC * kSP;
-    float* Bm = Dm + kC * kSP;                  // (do U^T) . D
+    float* dSs = Xs + kC * VP;                  // [DKP][VP]
+    float* Bm = dSs + DKP * VP;                 // (do U^T) . D
     float* Zm = Bm + kC * kSP;                  // Z + Z^T
-    float* red = Zm + kC * kSP;                 // [3][4][16]: dbeta, v.dv, q.dq by wave; [4]: <dS, S>
-    ChunkVec& cv = *reinterpret_cast<ChunkVec*>(red + 3 * 64 + 4);
+    float* redb = Zm + kC * kSP;                // [2][3][NW][16]: dbeta, v.dv, q.dq by wave
+    float* dotb = redb + 2 * 3 * NW * 16;       // [2][NW]: <dS, S> at the chunk's end
+    ChunkTiles* tiles = reinterpret_cast<ChunkTiles*>(dotb + 2 * NW);       // [2]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = lane & 15, g4 = (lane >> 4) << 2;
     const long long bh = blockIdx.x, b = bh / p.H;
@@ -376,186 +438,287 @@ __global__ __launch_bounds__(256) void delta_bwd_k(const Seq p) {
     const E* v = reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2];
     const E* dou = reinterpret_cast<const E*>(p.dout) + b * p.sdo[1] + h * p.sdo[2];
     const long long sst = (long long)p.DK * p.DV, st = p.B * p.H;
-
-    f4 dS[TPW][DKT], Sn[TPW][DKT];              // d(state after the chunk), state after the chunk
+    const unsigned srow = 4u * p.DV;
+    const float* ck0 = p.ckpt + bh * (p.nchunk + 1) * sst;
+    unsigned soff[TPW];
 #pragma unroll
     for (int w = 0; w < TPW; ++w) {
-        const int col = (wave + w * kMaxWaves) * 16 + li;
+        const int col = (wave + w * NW) * 16 + li;
+        soff[w] = col < p.DV ? 4u * (g4 * p.DV + col) : kOutside;
+    }
+
+    f4 dS[TPW][DKT], S0[TPW][DKT];              // d(state after the chunk); state before the chunk
+    E vnext[TPW][4];
+    RowTile<E, kC, DKP, 64 * NW, VEC> rk, rq;
+    RowTile<E, kC, DVP, 64 * NW, VEC> ro;
+    Gate gate;
+    auto valid_of = [&](int c) {
+        const long long left = p.T - (long long)c * kC;
+        return left < kC ? (int)left : kC;
+    };
+    auto fetch_state = [&](int c) {
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p);
 #pragma unroll
-        for (int t = 0; t < DKT; ++t)
+        for (int w = 0; w < TPW; ++w)
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S0[w][t][r] = state_load(rs, soff[w] + (16 * t + r) * srow);
+    };
+    auto fetch_v = [&](int c) {
+#pragma unroll
+        for (int w = 0; w < TPW; ++w) {
+            const int col = (wave + w * NW) * 16 + li;
+            const E* pv = v + (col < p.DV ? col : 0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int d = 16 * t + g4 + r;
-                const bool in = d < p.DK && col < p.DV;
-                const long long at = (long long)d * p.DV + col;
-                dS[w][t][r] = (in && p.dstate1) ? p.dstate1[bh * sst + at] : 0.f;
-                Sn[w][t][r] = in ? p.ckpt[(bh * (p.nchunk + 1) + p.nchunk) * sst + at] : 0.f;
+                const long long t = (long long)c * kC + g4 + r;
+                vnext[w][r] = pv[(t < p.T ? t : p.T - 1) * p.sv[0]];
             }
-    }
-    for (int c = p.nchunk - 1; c >= 0; --c) {
+        }
+    };
+    auto fetch_rows = [&](int c) {
         const long long t0 = (long long)c * kC;
-        const long long left = p.T - t0;
-        const int valid = left < kC ? (int)left : kC;
-        const float* ck = p.ckpt + (bh * (p.nchunk + 1) + c) * sst;
-        __syncthreads();
-        load_rows<E>(Ks, KP, k + t0 * p.sk[0], p.sk[0], kC, valid, p.DK, DKP, p.vec, 1.f);
-        load_rows<E>(Qs, KP, q + t0 * p.sq[0], p.sq[0], kC, valid, p.DK, DKP, p.vec, 1.f);
-        load_rows<E>(Os, VP, dou + t0 * p.sdo[0], p.sdo[0], kC, valid, p.DV, DVP, p.vec, p.scale);
-        __syncthreads();
-        if (wave == 0) {
-            double run; int seg;
-            chunk_gates(p, b, h, t0, lane, run, seg, &cv);
-            const f4 D = chunk_decay(run, seg, lane);
-            f4 kk = zero4(), qk = zero4();
-            const float* kr = Ks + li * KP + g4;
-            const float* qr = Qs + li * KP + g4;
+        const int valid = valid_of(c);
+        rk.issue(k + t0 * p.sk[0], p.sk[0], valid, p.DK);
+        rq.issue(q + t0 * p.sq[0], p.sq[0], valid, p.DK);
+        ro.issue(dou + t0 * p.sdo[0], p.sdo[0], valid, p.DV);
+        gate = load_gate(p, b, h, t0 + li);
+    };
+    auto commit_rows = [&](int c) {
+        const int valid = valid_of(c), par = c & 1;
+        rk.commit(Kb + par * kC * KP, KP, valid, p.DK, 1.f);
+        rq.commit(Qb + par * kC * KP, KP, valid, p.DK, 1.f);
+        ro.commit(Ob + par * kC * VP, VP, valid, p.DV, p.scale);
+    };
+    // the state-free part of chunk c, by two waves: `part` 0 gates, K K^T, inverse; 1: Q K^T
+    auto prepare = [&](int c, int part, const Gate& gt) {
+        ChunkTiles& ct = tiles[c & 1];
+        double run; int seg;
+        ChunkVec dump;
+        if (part == 0) chunk_gates(gt, lane, run, seg, &ct.cv);
+        else chunk_gates(gt, lane, run, seg, &dump);
+        const f4 D = chunk_decay(run, seg, lane);
+        const float* kr = Kb + (c & 1) * kC * KP + li * KP + g4;
+        const float* lr = part == 0 ? kr : Qb + (c & 1) * kC * KP + li * KP + g4;
+        f4 m0 = zero4(), m1 = zero4();
 #pragma unroll
-            for (int t = 0; t < DKT; ++t) {
-                const f4 a = lds4(kr + 16 * t), e = lds4(qr + 16 * t);
+        for (int t = 0; t < DKT; ++t) {
+            const f4 a = lds4(lr + 16 * t), e = lds4(kr + 16 * t);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) { kk = mfma(a[r], a[r], kk); qk = mfma(e[r], a[r], qk); }
-            }
+            for (int r = 0; r < 4; r += 2) { m0 = mfma(a[r], e[r], m0); m1 = mfma(a[r + 1], e[r + 1], m1); }
+        }
+        m0 = m0 + m1;
+        if (part == 0) {
             wave_sync();
+            const f4 be = lds4(ct.cv.beta + g4);
+            f4 L;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = g4 + r;
-                const float n = i > li ? D[r] * kk[r] : 0.f;
-                Nm[i * kSP + li] = n;
-                Ti[i * kSP + li] = cv.beta[i] * n;
-                Am[i * kSP + li] = i >= li ? D[r] * qk[r] : 0.f;
-                Dm[i * kSP + li] = D[r];
+                const float n = i > li ? D[r] * m0[r] : 0.f;
+                ct.Nm[i * kSP + li] = n;
+                ct.Dm[i * kSP + li] = D[r];
+                L[r] = be[r] * n;
             }
-            wave_sync();
-            unit_lower_inverse(Ti, lane);
+            unit_lower_inverse(L, ct.Ti, lane);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ct.Am[(g4 + r) * kSP + li] = g4 + r >= li ? D[r] * m0[r] : 0.f;
         }
+    };
+    auto dot_state = [&](int par) {             // this wave's part of <dS, S0> -> dotb[par]
+        float d = 0.f;
+#pragma unroll
+        for (int w = 0; w < TPW; ++w)
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) d += dS[w][t][r] * S0[w][t][r];
+        d = wave_sum(d);
+        if (lane == 0) dotb[par * NW + wave] = d;
+    };
+
+#pragma unroll
+    for (int w = 0; w < TPW; ++w)
+#pragma unroll
+        for (int t = 0; t < DKT; ++t) dS[w][t] = zero4();
+    if (p.dstate1) {
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.dstate1 + bh * sst, p);
+#pragma unroll
+        for (int w = 0; w < TPW; ++w)
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dS[w][t][r] = state_load(rs, soff[w] + (16 * t + r) * srow);
+    }
+    const int last = p.nchunk - 1;
+    if (last >= 0) {
+        fetch_rows(last);
+        fetch_state(p.nchunk);
+        dot_state(last & 1);
+        commit_rows(last);
+        const Gate gt = gate;
         __syncthreads();
-        const f4 be = lds4(cv.beta + g4), ga = lds4(cv.gam + g4), de = lds4(cv.toend + g4);
-        const float ge = cv.gend;
-        float db[4] = {0.f, 0.f, 0.f, 0.f}, vd[4] = {0.f, 0.f, 0.f, 0.f}, dots = 0.f;
+        fetch_state(last);
+        fetch_v(last);
+        if (last > 0) fetch_rows(last - 1);
+        if (wave >= 2 && wave < 4) prepare(last, wave - 2, gt);
+        __syncthreads();
+    }
+#pragma unroll 1
+    for (int c = last; c >= 0; --c) {
+        const long long t0 = (long long)c * kC;
+        const int par = c & 1;
+        const float* Ks = Kb + par * kC * KP;
+        const float* Qs = Qb + par * kC * KP;
+        const float* Os = Ob + par * kC * VP;
+        const ChunkTiles& ct = tiles[par];
+        float* red = redb + par * 3 * NW * 16;
+        const Gate gnext = gate;
+        if (c > 0) commit_rows(c - 1);
+        if (c > 1) fetch_rows(c - 2);
+        const f4 be = lds4(ct.cv.beta + g4), ga = lds4(ct.cv.gam + g4), de = lds4(ct.cv.toend + g4);
+        const float ge = ct.cv.gend;
+        float db[4] = {0.f, 0.f, 0.f, 0.f}, vd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < TPW; ++w) {
-            const int tile = wave + w * kMaxWaves, col = tile * 16 + li;
+            const int tile = wave + w * NW, col = tile * 16 + li;
             if (tile >= DVT) continue;
             const bool mine = col < p.DV;
             f4 vv, dd;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const long long t = t0 + g4 + r;
-                vv[r] = (mine && t < p.T) ? Elem<E>::get(v[t * p.sv[0] + col]) : 0.f;
+                vv[r] = mine && t0 + g4 + r < p.T ? Elem<E>::get(vnext[w][r]) : 0.f;
                 dd[r] = Os[(g4 + r) * VP + tile * 16 + li];
             }
 #pragma unroll
             for (int t = 0; t < DKT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * t + g4 + r;
-                    dots += dS[w][t][r] * Sn[w][t][r];
-                    Sn[w][t][r] = (d < p.DK && mine) ? ck[(long long)d * p.DV + col] : 0.f;
-                    dSs[d * VP + tile * 16 + li] = dS[w][t][r];
-                }
+                for (int r = 0; r < 4; ++r) dSs[(16 * t + g4 + r) * VP + tile * 16 + li] = dS[w][t][r];
             f4 ks = zero4(), kd = zero4();
             const float* kr = Ks + li * KP + g4;
 #pragma unroll
             for (int t = 0; t < DKT; ++t) {
                 const f4 a = lds4(kr + 16 * t);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) { ks = mfma(a[r], Sn[w][t][r], ks); kd = mfma(a[r], dS[w][t][r], kd); }
+                for (int r = 0; r < 4; ++r) { kd = mfma(a[r], dS[w][t][r], kd); ks = mfma(a[r], S0[w][t][r], ks); }
             }
-            f4 rhat, rhs, u = zero4(), y = zero4(), x, rres;
+            f4 rhat, rhs, u = zero4(), y = zero4(), x;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 rhat[r] = vv[r] - (ga[r] == 0.f ? 0.f : ga[r] * ks[r]);
                 rhs[r] = be[r] * rhat[r];
                 kd[r] *= de[r];
             }
-            const f4 ti = lds4(Ti + li * kSP + g4), nm = lds4(Nm + li * kSP + g4);
+            const f4 ti = lds4(ct.Ti + li * kSP + g4), nm = lds4(ct.Nm + li * kSP + g4);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) u = mfma(ti[r], rhs[r], u);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) kd = mfma(Am[(g4 + r) * kSP + li], dd[r], kd);           // dU
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y = mfma(Ti[(g4 + r) * kSP + li], kd[r], y);
+            for (int r = 0; r < 4; ++r) {
+                kd = mfma(ct.Am[(g4 + r) * kSP + li], dd[r], kd);            // dU
+                u = mfma(ti[r], rhs[r], u);
+            }
             f4 nu = zero4();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) nu = mfma(nm[r], u[r], nu);
+            for (int r = 0; r < 4; ++r) {
+                y = mfma(ct.Ti[(g4 + r) * kSP + li], kd[r], y);
+                nu = mfma(nm[r], u[r], nu);
+            }
+            E* dv = reinterpret_cast<E*>(p.dv) + ((t0 + g4) * st + bh) * p.DV + col;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 x[r] = be[r] * y[r];
-                rres[r] = rhat[r] - nu[r];
-                db[r] += y[r] * rres[r];
+                db[r] += y[r] * (rhat[r] - nu[r]);
                 vd[r] += vv[r] * x[r];
                 Us[(g4 + r) * VP + tile * 16 + li] = u[r];
                 Xs[(g4 + r) * VP + tile * 16 + li] = x[r];
-                const long long t = t0 + g4 + r;
-                if (mine && t < p.T) reinterpret_cast<E*>(p.dv)[(t * st + bh) * p.DV + col] = Elem<E>::put(x[r]);
+                if (mine && t0 + g4 + r < p.T) dv[r * st * p.DV] = Elem<E>::put(x[r]);
                 dd[r] *= ga[r];
                 x[r] = ga[r] == 0.f ? 0.f : -ga[r] * x[r];
             }
             const float* kc = Ks + g4 * KP + li;
             const float* qc = Qs + g4 * KP + li;
 #pragma unroll
-            for (int t = 0; t < DKT; ++t) {
+            for (int t = 0; t < DKT; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) dS[w][t][r] = ge == 0.f ? 0.f : ge * dS[w][t][r];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    dS[w][t] = mfma(qc[r * KP + 16 * t], dd[r], dS[w][t]);
-                    dS[w][t] = mfma(kc[r * KP + 16 * t], x[r], dS[w][t]);
-                }
-            }
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < DKT; ++t) dS[w][t] = mfma(qc[r * KP + 16 * t], dd[r], dS[w][t]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < DKT; ++t) dS[w][t] = mfma(kc[r * KP + 16 * t], x[r], dS[w][t]);
         }
+        dot_state(par ^ 1);                     // for the chunk before this one
+        if (c > 0) { fetch_state(c - 1); fetch_v(c - 1); }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             db[r] = row_sum(db[r]);
             vd[r] = row_sum(vd[r]);
-            if (li == 0) { red[wave * 16 + g4 + r] = db[r]; red[64 + wave * 16 + g4 + r] = vd[r]; }
+            if (li == 0) { red[wave * 16 + g4 + r] = db[r]; red[(NW + wave) * 16 + g4 + r] = vd[r]; }
         }
-        dots = wave_sum(dots);
-        if (lane == 0) red[192 + wave] = dots;
         __syncthreads();
         if (wave < 2) {         // wave 0: do U^T, wave 1: X U^T
             const float* ar = (wave == 0 ? Os : Xs) + li * VP + g4;
             const float* ur = Us + li * VP + g4;
-            f4 m = zero4();
+            f4 m0 = zero4(), m1 = zero4();
 #pragma unroll
             for (int t = 0; t < DVT; ++t) {
                 const f4 a = lds4(ar + 16 * t), e = lds4(ur + 16 * t);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) m = mfma(a[r], e[r], m);
+                for (int r = 0; r < 4; r += 2) { m0 = mfma(a[r], e[r], m0); m1 = mfma(a[r + 1], e[r + 1], m1); }
             }
+            m0 = m0 + m1;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = g4 + r;
-                const float D = Dm[i * kSP + li];
+                const float D = ct.Dm[i * kSP + li];
                 if (wave == 0) {
-                    Bm[i * kSP + li] = i >= li ? D * m[r] : 0.f;
-                } else if (i > li) {
-                    const float z = -D * m[r];
+                    Bm[i * kSP + li] = i >= li ? D * m0[r] : 0.f;
+                } else if (i >= li) {
+                    const float z = i > li ? -D * m0[r] : 0.f;
                     Zm[i * kSP + li] = z;
                     Zm[li * kSP + i] = z;
-                } else if (i == li) {
-                    Zm[i * kSP + li] = 0.f;
                 }
             }
+        } else if (wave < 4 && c > 0) {
+            prepare(c - 1, wave - 2, gnext);
         }
         __syncthreads();
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p);
         float qd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < KPW; ++w) {
-            const int tile = wave + w * kMaxWaves, kcol = tile * 16 + li;
+            const int tile = wave + w * NW, kcol = tile * 16 + li;
             if (tile >= DKT) continue;
             const bool mine = kcol < p.DK;
             f4 gq = zero4(), gu = zero4(), gx = zero4();
+            f4 s[DVT];
+            // (a piece that ends behind DV meets zero columns of do and X; rows behind DK read 0)
+#pragma unroll
+            for (int t = 0; t < DVT; ++t) {
+                const unsigned off = (unsigned)kcol * srow + 4u * (16 * t + g4);
+                if constexpr (VEC) {
+                    s[t] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[t][r] = state_load(rs, off + 4 * r);
+                }
+            }
 #pragma unroll
             for (int t = 0; t < DVT; ++t) {
                 const int c4 = 16 * t + g4;
-                f4 s;
+                const f4 e = lds4(dSs + kcol * VP + c4), uu = lds4(Us + li * VP + c4);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[r] = (mine && c4 + r < p.DV) ? ck[(long long)kcol * p.DV + c4 + r] : 0.f;
-                const f4 e = lds4(dSs + kcol * VP + c4);
-                const f4 od = lds4(Os + li * VP + c4), uu = lds4(Us + li * VP + c4), xx = lds4(Xs + li * VP + c4);
+                for (int r = 0; r < 4; ++r) gu = mfma(uu[r], e[r], gu);
+            }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) { gq = mfma(od[r], s[r], gq); gu = mfma(uu[r], e[r], gu); gx = mfma(xx[r], s[r], gx); }
+            for (int t = 0; t < DVT; ++t) {
+                const int c4 = 16 * t + g4;
+                const f4 od = lds4(Os + li * VP + c4), xx = lds4(Xs + li * VP + c4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) { gq = mfma(od[r], s[t][r], gq); gx = mfma(xx[r], s[t][r], gx); }
             }
             const f4 bm = lds4(Bm + li * kSP + g4), zm = lds4(Zm + li * kSP + g4);
             f4 dq, dk;
@@ -571,17 +734,18 @@ __global__ __launch_bounds__(256) void delta_bwd_k(const Seq p) {
                 dk = mfma(Bm[(g4 + r) * kSP + li], qv, dk);
                 dk = mfma(zm[r], kv, dk);
             }
+            const long long at = ((t0 + g4) * st + bh) * p.DK + kcol;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 qd[r] += dq[r] * Qs[(g4 + r) * KP + kcol];
-                const long long t = t0 + g4 + r;
-                if (mine && t < p.T) {
+                if (mine && t0 + g4 + r < p.T) {
+                    const long long i = at + r * st * p.DK;
                     if (p.dq32) {       // heads that share a key head: summed afterwards, in a fixed order
-                        p.dq32[(t * st + bh) * p.DK + kcol] = dq[r];
-                        p.dk32[(t * st + bh) * p.DK + kcol] = dk[r];
+                        p.dq32[i] = dq[r];
+                        p.dk32[i] = dk[r];
                     } else {
-                        reinterpret_cast<E*>(p.dq)[(t * st + bh) * p.DK + kcol] = Elem<E>::put(dq[r]);
-                        reinterpret_cast<E*>(p.dk)[(t * st + bh) * p.DK + kcol] = Elem<E>::put(dk[r]);
+                        reinterpret_cast<E*>(p.dq)[i] = Elem<E>::put(dq[r]);
+                        reinterpret_cast<E*>(p.dk)[i] = Elem<E>::put(dk[r]);
                     }
                 }
             }
@@ -589,18 +753,18 @@ __global__ __launch_bounds__(256) void delta_bwd_k(const Seq p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             qd[r] = row_sum(qd[r]);
-            if (li == 0) red[128 + wave * 16 + g4 + r] = qd[r];
+            if (li == 0) red[(2 * NW + wave) * 16 + g4 + r] = qd[r];
         }
         __syncthreads();
-        if (wave == 0) {
+        if (wave == 0) {        // (the others go on: red, dotb and the tiles alternate)
             float sb = 0.f, w = 0.f, dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < kMaxWaves; ++i) {
+            for (int i = 0; i < NW; ++i) {
                 sb += red[i * 16 + li];
-                w += red[128 + i * 16 + li] - red[64 + i * 16 + li];
-                dot += red[192 + i];
+                w += red[(2 * NW + i) * 16 + li] - red[(NW + i) * 16 + li];
+                dot += dotb[par * NW + i];
             }
-            const float sraw = cv.seg[li];
+            const float sraw = ct.cv.seg[li];
             const bool cut = sraw < 0.f;
             const float seg = cut ? -1.f - sraw : sraw;
             const float send = __shfl(seg, 15, 16);
@@ -618,17 +782,15 @@ __global__ __launch_bounds__(256) void delta_bwd_k(const Seq p) {
         }
     }
     if (p.dstate0) {
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.dstate0 + bh * sst, p);
 #pragma unroll
-        for (int w = 0; w < TPW; ++w) {
-            const int col = (wave + w * kMaxWaves) * 16 + li;
+        for (int w = 0; w < TPW; ++w)
+            if (wave + w * NW < DVT) {
 #pragma unroll
-            for (int t = 0; t < DKT; ++t)
+                for (int t = 0; t < DKT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int d = 16 * t + g4 + r;
-                    if (d < p.DK && col < p.DV) p.dstate0[bh * sst + (long long)d * p.DV + col] = dS[w][t][r];
-                }
-        }
+                    for (int r = 0; r < 4; ++r) state_store(dS[w][t][r], rs, soff[w] + (16 * t + r) * srow);
+            }
     }
 }
 
@@ -656,7 +818,7 @@ __global__ __launch_bounds__(256) void delta_fold_k(const float* __restrict__ a,
 template <typename E, int R, int VEC>
 __global__ __launch_bounds__(256) void delta_step_k(const Seq p, int slices) {
     const int lane = threadIdx.x & 63;
-    const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long w = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long bh = w / slices;
     if (bh >= p.B * p.H) return;
     const long long b = bh / p.H;
@@ -665,68 +827,68 @@ __global__ __launch_bounds__(256) void delta_step_k(const Seq p, int slices) {
     const bool mine = col < p.DV;
     const E* q = reinterpret_cast<const E*>(p.q) + b * p.sq[1] + hk * p.sq[2];
     const E* k = reinterpret_cast<const E*>(p.k) + b * p.sk[1] + hk * p.sk[2];
-    const E* v = reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2];
+    const E* v = reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2] + (mine ? col : 0);
     const long long sst = (long long)p.DK * p.DV;
-    const float* s0 = p.state0 + bh * sst + col;
-    float* s1 = p.state_out + bh * sst + col;
+    const __amdgpu_buffer_rsrc_t r0 = state_rsrc(p.state0 + bh * sst, p), r1 = state_rsrc(p.state_out + bh * sst, p);
+    const unsigned off = mine ? 4u * (grp * p.DV + col) : kOutside, srow = 16u * p.DV;     // row 4 i + grp: off + i * srow
     float S[R][VEC];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int d = 4 * i + grp;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) S[i][e] = 0.f;
-        if (mine && d < p.DK) {
-            if constexpr (VEC == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(s0 + (long long)d * p.DV);
-                S[i][0] = x.x; S[i][1] = x.y; S[i][2] = x.z; S[i][3] = x.w;
-            } else {
-                S[i][0] = s0[(long long)d * p.DV];
-            }
+        if constexpr (VEC == 4) {
+            const f4 x = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r0, off + i * srow, 0, 0));
+            S[i][0] = x[0]; S[i][1] = x[1]; S[i][2] = x[2]; S[i][3] = x[3];
+        } else {
+            S[i][0] = state_load(r0, off + i * srow);
         }
     }
     float kr[R], qr[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int d = 4 * i + grp;
-        kr[i] = d < p.DK ? Elem<E>::get(k[d]) : 0.f;
-        qr[i] = d < p.DK ? Elem<E>::get(q[d]) : 0.f;
+        const int d = 4 * i + grp, dc = d < p.DK ? d : 0;
+        kr[i] = Elem<E>::get(k[dc]);
+        qr[i] = Elem<E>::get(q[dc]);
+        if (d >= p.DK) kr[i] = qr[i] = 0.f;
     }
+    float vv[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) vv[e] = Elem<E>::get(v[e]);
     const float g = p.g[b * p.sg[1] + h * p.sg[2]], be = p.beta[b * p.sb[1] + h * p.sb[2]];
     const bool cut = (p.masks && p.masks[b * p.sm[1]] == 0.f) || g < kDead;
     const float al = expf(g);
-    float u[VEC], oo[VEC];
+    float oo[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        float acc = 0.f;
+        float a0 = 0.f, a1 = 0.f;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             S[i][e] = cut ? 0.f : al * S[i][e];
-            acc += kr[i] * S[i][e];
+            (i & 1 ? a1 : a0) += kr[i] * S[i][e];
         }
+        float acc = a0 + a1;
         acc += __shfl_xor(acc, 16, 64);
         acc += __shfl_xor(acc, 32, 64);
-        const float vv = mine ? Elem<E>::get(v[col + e]) : 0.f;
-        u[e] = be * (vv - acc);
-        float o = 0.f;
+        const float u = be * (vv[e] - acc);
+        a0 = a1 = 0.f;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            S[i][e] += kr[i] * u[e];
-            o += qr[i] * S[i][e];
+            S[i][e] += kr[i] * u;
+            (i & 1 ? a1 : a0) += qr[i] * S[i][e];
         }
+        float o = a0 + a1;
         o += __shfl_xor(o, 16, 64);
         o += __shfl_xor(o, 32, 64);
         oo[e] = o * p.scale;
     }
-    if (!mine) return;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int d = 4 * i + grp;
-        if (d < p.DK) {
-            if constexpr (VEC == 4) *reinterpret_cast<float4*>(s1 + (long long)d * p.DV) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
-            else s1[(long long)d * p.DV] = S[i][0];
+        if constexpr (VEC == 4) {
+            const f4 x = {S[i][0], S[i][1], S[i][2], S[i][3]};
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, x), r1, off + i * srow, 0, 0);
+        } else {
+            state_store(S[i][0], r1, off + i * srow);
         }
     }
-    if (grp == 0) {
+    if (mine && grp == 0) {
         E* o = reinterpret_cast<E*>(p.o) + bh * p.DV + col;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) o[e] = Elem<E>::put(oo[e]);
@@ -745,8 +907,9 @@ const char* sizes_error(const dcc_delta_seq* s) {
     if (s->T > (1ll << 31) || (double)s->B * s->H > 2147483647.0) return "more than 2^31 tokens or (row, head) pairs";
     return nullptr;
 }
-bool rows_vec(const void* p, const long long* st, int dtype) {
-    return aligned(p, 4 * esize(dtype)) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+// rows of `dim` elements that may be read four at a time
+bool rows_vec(const void* p, const long long* st, int dim, int dtype) {
+    return aligned(p, 4 * esize(dtype)) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0 && dim % 4 == 0;
 }
 Seq base(const dcc_delta_seq* s) {
     Seq p = {};
@@ -757,7 +920,7 @@ Seq base(const dcc_delta_seq* s) {
     for (int i = 0; i < 3; ++i) { p.sq[i] = s->st_q[i]; p.sk[i] = s->st_k[i]; p.sv[i] = s->st_v[i]; p.sg[i] = s->st_g[i]; p.sb[i] = s->st_beta[i]; }
     for (int i = 0; i < 2; ++i) p.sm[i] = s->st_masks[i];
     p.o = s->o; p.state_out = s->state1; p.ckpt = s->ckpt;
-    p.vec = rows_vec(s->q, p.sq, s->dtype) && rows_vec(s->k, p.sk, s->dtype);
+    p.vec = rows_vec(s->q, p.sq, s->DK, s->dtype) && rows_vec(s->k, p.sk, s->DK, s->dtype);
     return p;
 }
 int done(const char* what) {
@@ -772,34 +935,41 @@ bool allow_lds(K kernel, size_t bytes) {
     return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
 }
 
-template <typename E, int DKT, int BT>
+template <typename E, int DKT, int BT, int NW, bool VEC>
 int launch_fwd(const Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4;
     const size_t lds = sizeof(float) * (2 * BT * kC * KP + 2 * BT * kC * kSP) + BT * sizeof(ChunkVec);
-    const int nt = (p.DV + 15) / 16, nw = nt < kMaxWaves ? nt : kMaxWaves;
-    if (!allow_lds(delta_fwd_k<E, DKT, BT>, lds)) return dcc_fail(kEHIP, "dcc_delta_fwd: shared memory refused");
-    hipLaunchKernelGGL((delta_fwd_k<E, DKT, BT>), dim3((unsigned)(p.B * p.H), (nt + nw - 1) / nw), dim3(64 * nw), lds, st, p);
+    const int nt = (p.DV + 15) / 16;
+    if (!allow_lds(delta_fwd_k<E, DKT, BT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_fwd: shared memory refused");
+    hipLaunchKernelGGL((delta_fwd_k<E, DKT, BT, NW, VEC>), dim3((unsigned)(p.B * p.H), (nt + NW - 1) / NW), dim3(64 * NW), lds, st, p);
     return done("dcc_delta_fwd");
+}
+template <typename E, int DKT>
+int fwd_dk(const Seq& p, hipStream_t st) {
+    if (!p.vec) return launch_fwd<E, DKT, 1, 4, false>(p, st);
+    if (p.nchunk <= 1) return p.DV <= 32 ? launch_fwd<E, DKT, 1, 2, true>(p, st) : launch_fwd<E, DKT, 1, 4, true>(p, st);
+    return p.DV <= 32 ? launch_fwd<E, DKT, 2, 2, true>(p, st) : launch_fwd<E, DKT, 4, 4, true>(p, st);
 }
 template <typename E>
 int fwd_typed(const Seq& p, hipStream_t st) {
     const int t = (p.DK + 15) / 16;
-    if (p.nchunk == 1) return t <= 2 ? launch_fwd<E, 2, 1>(p, st) : t <= 4 ? launch_fwd<E, 4, 1>(p, st) : launch_fwd<E, 8, 1>(p, st);
-    return t <= 2 ? launch_fwd<E, 2, 4>(p, st) : t <= 4 ? launch_fwd<E, 4, 4>(p, st) : launch_fwd<E, 8, 4>(p, st);
+    return t <= 2 ? fwd_dk<E, 2>(p, st) : t <= 4 ? fwd_dk<E, 4>(p, st) : fwd_dk<E, 8>(p, st);
 }
 
-template <typename E, int DKT, int DVT>
+template <typename E, int DKT, int DVT, int NW, bool VEC>
 int launch_bwd(const Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, VP = DVT * 16 + 4;
-    const size_t lds = sizeof(float) * (2 * kC * KP + 3 * kC * VP + DKT * 16 * VP + 6 * kC * kSP + 3 * 64 + 4) + sizeof(ChunkVec);
-    if (!allow_lds(delta_bwd_k<E, DKT, DVT>, lds)) return dcc_fail(kEHIP, "dcc_delta_bwd: shared memory refused");
-    hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT>), dim3((unsigned)(p.B * p.H)), dim3(64 * kMaxWaves), lds, st, p);
+    const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 6 * NW * 16 + 2 * NW) + 2 * sizeof(ChunkTiles);
+    if (!allow_lds(delta_bwd_k<E, DKT, DVT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_bwd: shared memory refused");
+    hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3((unsigned)(p.B * p.H)), dim3(64 * NW), lds, st, p);
     return done("dcc_delta_bwd");
 }
 template <typename E, int DKT>
 int bwd_dv(const Seq& p, hipStream_t st) {
     const int t = (p.DV + 15) / 16;
-    return t <= 2 ? launch_bwd<E, DKT, 2>(p, st) : t <= 4 ? launch_bwd<E, DKT, 4>(p, st) : launch_bwd<E, DKT, 8>(p, st);
+    constexpr int NW = DKT > 4 ? 8 : 4;
+    if (!p.vec) return launch_bwd<E, DKT, 8, 8, false>(p, st);
+    return t <= 2 ? launch_bwd<E, DKT, 2, NW, true>(p, st) : t <= 4 ? launch_bwd<E, DKT, 4, NW, true>(p, st) : launch_bwd<E, DKT, 8, 8, true>(p, st);
 }
 template <typename E>
 int bwd_typed(const Seq& p, hipStream_t st) {
@@ -825,7 +995,7 @@ int step_rows(const Seq& p, hipStream_t st) {
 }
 template <typename E>
 int step_typed(const Seq& p, hipStream_t st) {
-    return p.DK <= 32 ? step_rows<E, 8>(p, st) : p.DK <= 64 ? step_rows<E, 16>(p, st) : step_rows<E, 32>(p, st);
+    return p.DK <= 32 ? step_rows<E, 8>(p, st) : p.DK <= 64 ? step_rows<E, 16>(p, st) : p.DK <= 96 ? step_rows<E, 24>(p, st) : step_rows<E, 32>(p, st);
 }
 
 }  // namespace
@@ -872,7 +1042,7 @@ DCC_API int dcc_delta_bwd(const dcc_delta_seq* s, const dcc_delta_grad* d, float
     p.dout = d->dout; p.dstate1 = d->dstate1; p.ckpt = const_cast<float*>(d->ckpt);
     for (int i = 0; i < 3; ++i) p.sdo[i] = d->st_do[i];
     p.dq = d->dq; p.dk = d->dk; p.dv = d->dv; p.dg = d->dg; p.dbeta = d->dbeta; p.dstate0 = d->dstate0;
-    p.vec = p.vec && rows_vec(d->dout, p.sdo, s->dtype);
+    p.vec = p.vec && rows_vec(d->dout, p.sdo, s->DV, s->dtype);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     switch (s->dtype) {
         case DCC_DELTA_F32: return bwd_typed<float>(p, st);
