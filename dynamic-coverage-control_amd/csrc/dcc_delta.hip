@@ -17,6 +17,7 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -29,6 +30,7 @@ namespace {
 
 constexpr int kEINVAL = -1, kEHIP = -2;
 constexpr int kC = 16;                  // tokens per chunk
+constexpr int64_t kSegBelow = 128, kSegFill = 512, kSegMin = 16;      // segments of long sequences: see segments_of
 constexpr float kDead = -103.98f;       // exp() below this is 0 in float32: a restart
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -70,6 +72,8 @@ struct Seq {        // dcc_delta_seq / dcc_delta_grad as the kernels read them
     float *state_out, *ckpt, *dq32, *dk32;
     void *dq, *dk, *dv;
     float *dg, *dbeta, *dstate0;
+    int nseg, seglen;            // the chunks in segments of `seglen` (a multiple of the block) that run side by side; nseg 1: one
+    float *sumN, *sumP, *segS;   // [nseg - 1] segment summaries N [DK, DV], P [DK, DK]; [nseg] states at segment starts (all per (row, head))
     int vec;        // rows of q, k (and dout, v) may be read four elements at a time
 };
 
@@ -96,8 +100,8 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // A state [DK, DV] through a buffer descriptor: 32-bit offsets, rows and columns outside it read 0 and write nothing.
 constexpr unsigned kOutside = 0x40000000u;      // byte offset of lanes without a column
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t state_rsrc(const float* base, const Seq& p) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, p.DK * p.DV * 4, 0x00027000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t state_rsrc(const float* base, int rows, int cols) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), 0, rows * cols * 4, 0x00027000);
 }
 __device__ __forceinline__ float state_load(__amdgpu_buffer_rsrc_t rs, unsigned off) {
     return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
@@ -221,19 +225,21 @@ __device__ __forceinline__ void unit_lower_inverse(const f4& L, float* t, int la
     }
 }
 
-// K K^T and Q K^T of one chunk from its LDS rows
-template <int DKT>
+// K K^T and (HASQ) Q K^T of one chunk from its LDS rows
+template <int DKT, bool HASQ>
 __device__ __forceinline__ void chunk_products(const float* kr, const float* qr, f4& kk, f4& qk) {
     f4 k0 = zero4(), k1 = zero4(), q0 = zero4(), q1 = zero4();
 #pragma unroll
     for (int t = 0; t < DKT; ++t) {
-        const f4 a = lds4(kr + 16 * t), e = lds4(qr + 16 * t);
+        const f4 a = lds4(kr + 16 * t);
+        f4 e = zero4();
+        if (HASQ) e = lds4(qr + 16 * t);
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
             k0 = mfma(a[r], a[r], k0);
-            q0 = mfma(e[r], a[r], q0);
+            if (HASQ) q0 = mfma(e[r], a[r], q0);
             k1 = mfma(a[r + 1], a[r + 1], k1);
-            q1 = mfma(e[r + 1], a[r + 1], q1);
+            if (HASQ) q1 = mfma(e[r + 1], a[r + 1], q1);
         }
     }
     kk = k0 + k1;
@@ -244,40 +250,65 @@ __device__ __forceinline__ void chunk_products(const float* kr, const float* qr,
 // One workgroup per (row, head) and NW tiles of 16 value columns; each wave keeps its [DK, 16] slice of the state in registers and
 // walks the chunks.  Blocks of BT chunks are staged in LDS: the waves first split the state-free part (K K^T, Q K^T, gates, inverse) of
 // the BT chunks among them, then every wave runs the BT chunks on its own columns without a barrier, while the next block is loading.
-template <typename E, int DKT, int BT, int NW, bool VEC>
+//
+// Few long sequences are cut into segments that run side by side.  A segment maps its start state S to P S + N: SUM_FWD runs it from
+// zero on the value columns (N) and from the identity on DK more (P), delta_join_k chains the segments, and FULL runs each from its
+// own start.  SUM_BWD does the same for d(state), which runs the other way: dS <- gam_C dS + Q^T (gam do) - K^T (gam X) needs no state.
+enum { FULL = 0, SUM_FWD = 1, SUM_BWD = 2 };
+
+template <typename E, int DKT, int BT, int NW, bool VEC, int MODE>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4 ? 2 : 3))) void delta_fwd_k(const Seq p) {
     constexpr int DKP = DKT * 16, KP = DKP + 4, CPW = (BT + NW - 1) / NW;
+    constexpr bool HASQ = MODE != SUM_FWD;
     extern __shared__ float sh[];
     float* Ks = sh;
-    float* Qs = Ks + BT * kC * KP;
-    float* Ti = Qs + BT * kC * KP;              // [BT][16][kSP] inverse
-    float* Am = Ti + BT * kC * kSP;             // [BT][16][kSP] (Q K^T) . D
-    ChunkVec* cvs = reinterpret_cast<ChunkVec*>(Am + BT * kC * kSP);
+    float* Ti = Ks + BT * kC * KP;              // [BT][16][kSP] inverse
+    ChunkVec* cvs = reinterpret_cast<ChunkVec*>(Ti + BT * kC * kSP);
+    float* Qs = reinterpret_cast<float*>(cvs + BT);
+    float* Am = Qs + BT * kC * KP;              // [BT][16][kSP] (Q K^T) . D
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int li = lane & 15, g4 = (lane >> 4) << 2;
     const long long bh = blockIdx.x, b = bh / p.H;
     const int h = (int)(bh - b * p.H), hk = h / p.rep;
-    const int tile = blockIdx.y * NW + wave, col = tile * 16 + li;
-    const bool live = tile * 16 < p.DV, mine = col < p.DV;
+    const int nt = (p.DV + 15) / 16, tile0 = blockIdx.y * NW + wave;
+    // (SUM_BWD leaves out segment 0, the others the last one)
+    const int seg = MODE == SUM_BWD ? blockIdx.z + 1 : blockIdx.z;
+    const bool unit = MODE != FULL && tile0 >= nt;              // a tile of the identity's columns
+    const int tile = unit ? tile0 - nt : tile0, col = tile * 16 + li, ncol = unit ? p.DK : p.DV;
+    const bool live = tile * 16 < ncol, mine = col < ncol, full = !unit && mine;
     const E* q = reinterpret_cast<const E*>(p.q) + b * p.sq[1] + hk * p.sq[2];
     const E* k = reinterpret_cast<const E*>(p.k) + b * p.sk[1] + hk * p.sk[2];
-    const E* v = reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2] + (mine ? col : 0);
+    const E* v = MODE == SUM_BWD ? reinterpret_cast<const E*>(p.dout) + b * p.sdo[1] + h * p.sdo[2] : reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2];
+    const long long sv0 = MODE == SUM_BWD ? p.sdo[0] : p.sv[0];
+    v += full ? col : 0;
     E* o = reinterpret_cast<E*>(p.o) + bh * (long long)p.DV + col;
     const long long so = p.B * p.H * (long long)p.DV, sst = (long long)p.DK * p.DV;
-    const unsigned srow = 4u * p.DV, soff = mine ? 4u * (g4 * p.DV + col) : kOutside;   // state element (16 t + 4 g + r, col): soff + (16 t + r) * srow
+    const unsigned srow = 4u * ncol, soff = mine ? 4u * (g4 * ncol + col) : kOutside;   // state element (16 t + 4 g + r, col): soff + (16 t + r) * srow
+    const int cbeg = seg * p.seglen, cend = cbeg + p.seglen < p.nchunk ? cbeg + p.seglen : p.nchunk;
 
     f4 S[DKT];
 #pragma unroll
     for (int t = 0; t < DKT; ++t) S[t] = zero4();
-    if (p.state0) {
-        const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.state0 + bh * sst, p);
+    {
+        const float* from = nullptr;
+        if (MODE == FULL) from = seg == 0 ? p.state0 ? p.state0 + bh * sst : nullptr : p.segS + (bh * p.nseg + seg) * sst;
+        if (MODE == SUM_FWD && !unit && seg == 0 && p.state0) from = p.state0 + bh * sst;
+        if (MODE == SUM_BWD && !unit && seg == p.nseg - 1 && p.dstate1) from = p.dstate1 + bh * sst;
+        if (from) {
+            const __amdgpu_buffer_rsrc_t rs = state_rsrc(from, p.DK, p.DV);
 #pragma unroll
-        for (int t = 0; t < DKT; ++t)
+            for (int t = 0; t < DKT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[t][r] = state_load(rs, soff + (16 * t + r) * srow);
+                for (int r = 0; r < 4; ++r) S[t][r] = state_load(rs, soff + (16 * t + r) * srow);
+        } else if (unit) {
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[t][r] = 16 * t + g4 + r == col ? 1.f : 0.f;
+        }
     }
     auto store_state = [&](float* base) {
-        const __amdgpu_buffer_rsrc_t rs = state_rsrc(base, p);
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(base, p.DK, ncol);
 #pragma unroll
         for (int t = 0; t < DKT; ++t)
 #pragma unroll
@@ -294,7 +325,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
         const long long t0 = (long long)c0 * kC;
         const int valid = valid_of(c0);
         rk.issue(k + t0 * p.sk[0], p.sk[0], valid, p.DK);
-        rq.issue(q + t0 * p.sq[0], p.sq[0], valid, p.DK);
+        if (HASQ) rq.issue(q + t0 * p.sq[0], p.sq[0], valid, p.DK);
 #pragma unroll
         for (int n = 0; n < CPW; ++n) gate[n] = load_gate(p, b, h, t0 + (wave + n * NW) * kC + li);
     };
@@ -302,78 +333,132 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const long long t = t0 + g4 + r;
-            vnext[r] = v[(t < p.T ? t : p.T - 1) * p.sv[0]];
+            vnext[r] = v[(t < p.T ? t : p.T - 1) * sv0];
         }
     };
-    if (p.nchunk > 0) { fetch(0); fetch_v(0); }
-    for (int c0 = 0; c0 < p.nchunk; c0 += BT) {
+    const int nblk = (cend - cbeg + BT - 1) / BT;
+    auto block = [&](int i) { return cbeg + BT * (MODE == SUM_BWD ? nblk - 1 - i : i); };
+    if (nblk > 0) {
+        fetch(block(0));
+        fetch_v((long long)(MODE == SUM_BWD ? cend - 1 : cbeg) * kC);
+    }
+    for (int i = 0; i < nblk; ++i) {
+        const int c0 = block(i);
         const long long t0 = (long long)c0 * kC;
-        const int nc = p.nchunk - c0 < BT ? p.nchunk - c0 : BT, valid = valid_of(c0);
+        const int nc = cend - c0 < BT ? cend - c0 : BT, valid = valid_of(c0);
         __syncthreads();
         rk.commit(Ks, KP, valid, p.DK, 1.f);
-        rq.commit(Qs, KP, valid, p.DK, 1.f);
+        if (HASQ) rq.commit(Qs, KP, valid, p.DK, 1.f);
         Gate now[CPW];
 #pragma unroll
         for (int n = 0; n < CPW; ++n) now[n] = gate[n];
         __syncthreads();
-        if (c0 + BT < p.nchunk) fetch(c0 + BT);
+        if (i + 1 < nblk) fetch(block(i + 1));
 #pragma unroll
         for (int n = 0; n < CPW; ++n) {
             const int c = wave + n * NW;
             if (c >= nc) continue;
-            double run; int seg;
-            chunk_gates(now[n], lane, run, seg, cvs + c);
-            const f4 D = chunk_decay(run, seg, lane);
+            double run; int sg;
+            chunk_gates(now[n], lane, run, sg, cvs + c);
+            const f4 D = chunk_decay(run, sg, lane);
             f4 kk, qk, L;
-            chunk_products<DKT>(Ks + (c * kC + li) * KP + g4, Qs + (c * kC + li) * KP + g4, kk, qk);
+            chunk_products<DKT, HASQ>(Ks + (c * kC + li) * KP + g4, Qs + (c * kC + li) * KP + g4, kk, qk);
             wave_sync();
             const f4 be = lds4(cvs[c].beta + g4);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = g4 + r;
-                L[r] = i > li ? be[r] * D[r] * kk[r] : 0.f;
-                Am[(c * kC + i) * kSP + li] = i >= li ? D[r] * qk[r] : 0.f;
+                const int j = g4 + r;
+                L[r] = j > li ? be[r] * D[r] * kk[r] : 0.f;
+                if (HASQ) Am[(c * kC + j) * kSP + li] = j >= li ? D[r] * qk[r] : 0.f;
             }
             unit_lower_inverse(L, Ti + c * kC * kSP, lane);
         }
         __syncthreads();
         if (live) {
 #pragma unroll 1
-            for (int c = 0; c < nc; ++c) {
+            for (int n = 0; n < nc; ++n) {
+                const int c = MODE == SUM_BWD ? nc - 1 - n : n;
                 const long long tc = t0 + c * kC;
                 f4 vv;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) vv[r] = mine && tc + g4 + r < p.T ? Elem<E>::get(vnext[r]) : 0.f;
-                if (c0 + c + 1 < p.nchunk) fetch_v(tc + kC);
-                if (p.ckpt) store_state(p.ckpt + (bh * (p.nchunk + 1) + c0 + c) * sst);
+                for (int r = 0; r < 4; ++r) vv[r] = full && tc + g4 + r < p.T ? Elem<E>::get(vnext[r]) : 0.f;
+                if (MODE == SUM_BWD ? c0 + c > cbeg : c0 + c + 1 < cend) fetch_v(MODE == SUM_BWD ? tc - kC : tc + kC);
+                if (MODE == FULL && p.ckpt) store_state(p.ckpt + (bh * (p.nchunk + 1) + c0 + c) * sst);
                 const float* kr = Ks + (c * kC + li) * KP + g4;
                 const float* qr = Qs + (c * kC + li) * KP + g4;
-                f4 ks = zero4(), qs = zero4();
-#pragma unroll
-                for (int t = 0; t < DKT; ++t) {
-                    const f4 a = lds4(kr + 16 * t), e = lds4(qr + 16 * t);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) { ks = mfma(a[r], S[t][r], ks); qs = mfma(e[r], S[t][r], qs); }
-                }
                 const ChunkVec& cv = cvs[c];
                 const f4 be = lds4(cv.beta + g4), ga = lds4(cv.gam + g4), de = lds4(cv.toend + g4);
+                const float ge = cv.gend;
+                const float* kc = Ks + (c * kC + g4) * KP + li;
+                const float* qc = Qs + (c * kC + g4) * KP + li;
+                f4 ks = zero4(), qs = zero4();
+                if (MODE == SUM_BWD) {
+                    // dU = A^T do + D_C K dS, Y = (I + beta N)^-T dU, dS <- gam_C dS + Q^T (gam do) - K^T (gam beta Y)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) vv[r] *= p.scale;
+#pragma unroll
+                    for (int t = 0; t < DKT; ++t) {
+                        const f4 a = lds4(kr + 16 * t);
+#pragma unroll
+                        for (int r = 0; r < 4; r += 2) { ks = mfma(a[r], S[t][r], ks); qs = mfma(a[r + 1], S[t][r + 1], qs); }
+                    }
+                    f4 y = zero4();
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) ks[r] = (ks[r] + qs[r]) * de[r];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) ks = mfma(Am[(c * kC + g4 + r) * kSP + li], vv[r], ks);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y = mfma(Ti[(c * kC + g4 + r) * kSP + li], ks[r], y);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        vv[r] *= ga[r];
+                        y[r] = ga[r] == 0.f ? 0.f : -ga[r] * (be[r] * y[r]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) S[t][r] = ge == 0.f ? 0.f : ge * S[t][r];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int t = 0; t < DKT; ++t) S[t] = mfma(qc[r * KP + 16 * t], vv[r], S[t]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int t = 0; t < DKT; ++t) S[t] = mfma(kc[r * KP + 16 * t], y[r], S[t]);
+                    continue;
+                }
+#pragma unroll
+                for (int t = 0; t < DKT; ++t) {
+                    const f4 a = lds4(kr + 16 * t);
+                    if (MODE == FULL) {
+                        const f4 e = lds4(qr + 16 * t);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) { ks = mfma(a[r], S[t][r], ks); qs = mfma(e[r], S[t][r], qs); }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; r += 2) { ks = mfma(a[r], S[t][r], ks); qs = mfma(a[r + 1], S[t][r + 1], qs); }
+                    }
+                }
+                if (MODE != FULL) ks += qs;
                 f4 rhs, out;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     rhs[r] = be[r] * (vv[r] - (ga[r] == 0.f ? 0.f : ga[r] * ks[r]));
                     out[r] = ga[r] == 0.f ? 0.f : ga[r] * qs[r];
                 }
-                const f4 ti = lds4(Ti + (c * kC + li) * kSP + g4), am = lds4(Am + (c * kC + li) * kSP + g4);
+                const f4 ti = lds4(Ti + (c * kC + li) * kSP + g4);
                 f4 u = zero4();
 #pragma unroll
                 for (int r = 0; r < 4; ++r) u = mfma(ti[r], rhs[r], u);
-                const float ge = cv.gend;
-                const float* kc = Ks + (c * kC + g4) * KP + li;
                 f4 ud;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) ud[r] = u[r] * de[r];
+                if (MODE == FULL) {
+                    const f4 am = lds4(Am + (c * kC + li) * kSP + g4);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) out = mfma(am[r], u[r], out);
+                    for (int r = 0; r < 4; ++r) out = mfma(am[r], u[r], out);
+                }
 #pragma unroll
                 for (int t = 0; t < DKT; ++t)
 #pragma unroll
@@ -382,21 +467,84 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int t = 0; t < DKT; ++t) S[t] = mfma(kc[r * KP + 16 * t], ud[r], S[t]);
-                E* oc = o + (tc + g4) * so;
-                if (mine && tc + kC <= p.T) {
+                if (MODE == FULL) {
+                    E* oc = o + (tc + g4) * so;
+                    if (mine && tc + kC <= p.T) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) oc[r * so] = Elem<E>::put(out[r] * p.scale);
-                } else if (mine) {
+                        for (int r = 0; r < 4; ++r) oc[r * so] = Elem<E>::put(out[r] * p.scale);
+                    } else if (mine) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (tc + g4 + r < p.T) oc[r * so] = Elem<E>::put(out[r] * p.scale);
+                        for (int r = 0; r < 4; ++r)
+                            if (tc + g4 + r < p.T) oc[r * so] = Elem<E>::put(out[r] * p.scale);
+                    }
                 }
             }
         }
     }
-    if (live) {
+    if (!live) return;
+    if (MODE != FULL) {
+        const long long at = bh * (p.nseg - 1) + blockIdx.z;
+        store_state(unit ? p.sumP + at * p.DK * p.DK : p.sumN + at * sst);
+    } else if (seg == p.nseg - 1) {
         if (p.state_out) store_state(p.state_out + bh * sst);
         if (p.ckpt) store_state(p.ckpt + (bh * (p.nchunk + 1) + p.nchunk) * sst);
+    }
+}
+
+// States at the segment starts from the segments' summaries: S <- P S + N, one 16-column tile per workgroup, wave w the rows 16 w..;
+// the state passes through LDS (one barrier a segment) while the next P and N are loading.  `back`: from the last segment to the first.
+template <int DKT>
+__global__ __launch_bounds__(64 * DKT) void delta_join_k(const Seq p, int back) {
+    __shared__ float sh[2][DKT * 16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g4 = (lane >> 4) << 2;
+    const long long bh = blockIdx.x, sst = (long long)p.DK * p.DV, spp = (long long)p.DK * p.DK;
+    const int col = blockIdx.y * 16 + li, n = p.nseg - 1;
+    const unsigned srow = 4u * p.DV, off = col < p.DV ? 4u * ((16 * wave + g4) * p.DV + col) : kOutside;
+    const int prow = 16 * wave + li;
+    f4 P[DKT], N;
+    // summary i belongs to segment i (forward) or i + 1 (backward)
+    auto fetch = [&](int i, bool withP) {
+        const __amdgpu_buffer_rsrc_t rn = state_rsrc(p.sumN + (bh * n + i) * sst, p.DK, p.DV), rp = state_rsrc(p.sumP + (bh * n + i) * spp, p.DK, p.DK);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) N[r] = state_load(rn, off + r * srow);
+        if (!withP) return;
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = 16 * t + g4 + r;
+                P[t][r] = state_load(rp, k < p.DK ? 4u * (prow * p.DK + k) : kOutside);
+            }
+    };
+    fetch(back ? n - 1 : 0, false);
+    f4 S = N;
+    for (int i = 0; i < n; ++i) {
+        float (*x)[17] = sh[i & 1];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[16 * wave + g4 + r][li] = S[r];
+        const int seg = back ? n - 1 - i : i + 1;       // the segment that this state enters
+        const __amdgpu_buffer_rsrc_t ro = state_rsrc(p.segS + (bh * p.nseg + seg) * sst, p.DK, p.DV);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) state_store(S[r], ro, off + r * srow);
+        if (i + 1 == n) break;
+        fetch(back ? n - 2 - i : i + 1, true);
+        __syncthreads();
+        // a segment with a restart has P == 0, and then what the state held before (NaN included) is gone: not multiplied
+        bool any = false;
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) any |= P[t][r] != 0.f;
+        if (!__any(any)) { S = N; continue; }
+        f4 a = N, c = zero4();
+#pragma unroll
+        for (int t = 0; t < DKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+                a = mfma(P[t][r], x[16 * t + g4 + r][li], a);
+                c = mfma(P[t][r + 1], x[16 * t + g4 + r + 1][li], c);
+            }
+        S = a + c;
     }
 }
 
@@ -440,6 +588,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     const long long sst = (long long)p.DK * p.DV, st = p.B * p.H;
     const unsigned srow = 4u * p.DV;
     const float* ck0 = p.ckpt + bh * (p.nchunk + 1) * sst;
+    const int seg = blockIdx.y, cbeg = seg * p.seglen, cend = cbeg + p.seglen < p.nchunk ? cbeg + p.seglen : p.nchunk;
     unsigned soff[TPW];
 #pragma unroll
     for (int w = 0; w < TPW; ++w) {
@@ -457,7 +606,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         return left < kC ? (int)left : kC;
     };
     auto fetch_state = [&](int c) {
-        const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p);
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p.DK, p.DV);
 #pragma unroll
         for (int w = 0; w < TPW; ++w)
 #pragma unroll
@@ -543,8 +692,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     for (int w = 0; w < TPW; ++w)
 #pragma unroll
         for (int t = 0; t < DKT; ++t) dS[w][t] = zero4();
-    if (p.dstate1) {
-        const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.dstate1 + bh * sst, p);
+    const float* from = seg == p.nseg - 1 ? p.dstate1 ? p.dstate1 + bh * sst : nullptr : p.segS + (bh * p.nseg + seg) * sst;
+    if (from) {
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(from, p.DK, p.DV);
 #pragma unroll
         for (int w = 0; w < TPW; ++w)
 #pragma unroll
@@ -552,22 +702,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
                 for (int r = 0; r < 4; ++r) dS[w][t][r] = state_load(rs, soff[w] + (16 * t + r) * srow);
     }
-    const int last = p.nchunk - 1;
-    if (last >= 0) {
+    const int last = cend - 1;
+    if (last >= cbeg) {
         fetch_rows(last);
-        fetch_state(p.nchunk);
+        fetch_state(cend);
         dot_state(last & 1);
         commit_rows(last);
         const Gate gt = gate;
         __syncthreads();
         fetch_state(last);
         fetch_v(last);
-        if (last > 0) fetch_rows(last - 1);
+        if (last > cbeg) fetch_rows(last - 1);
         if (wave >= 2 && wave < 4) prepare(last, wave - 2, gt);
         __syncthreads();
     }
 #pragma unroll 1
-    for (int c = last; c >= 0; --c) {
+    for (int c = last; c >= cbeg; --c) {
         const long long t0 = (long long)c * kC;
         const int par = c & 1;
         const float* Ks = Kb + par * kC * KP;
@@ -576,8 +726,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const ChunkTiles& ct = tiles[par];
         float* red = redb + par * 3 * NW * 16;
         const Gate gnext = gate;
-        if (c > 0) commit_rows(c - 1);
-        if (c > 1) fetch_rows(c - 2);
+        if (c > cbeg) commit_rows(c - 1);
+        if (c > cbeg + 1) fetch_rows(c - 2);
         const f4 be = lds4(ct.cv.beta + g4), ga = lds4(ct.cv.gam + g4), de = lds4(ct.cv.toend + g4);
         const float ge = ct.cv.gend;
         float db[4] = {0.f, 0.f, 0.f, 0.f}, vd[4] = {0.f, 0.f, 0.f, 0.f};
@@ -651,7 +801,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
                 for (int t = 0; t < DKT; ++t) dS[w][t] = mfma(kc[r * KP + 16 * t], x[r], dS[w][t]);
         }
         dot_state(par ^ 1);                     // for the chunk before this one
-        if (c > 0) { fetch_state(c - 1); fetch_v(c - 1); }
+        if (c > cbeg) { fetch_state(c - 1); fetch_v(c - 1); }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             db[r] = row_sum(db[r]);
@@ -682,11 +832,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
                     Zm[li * kSP + i] = z;
                 }
             }
-        } else if (wave < 4 && c > 0) {
+        } else if (wave < 4 && c > cbeg) {
             prepare(c - 1, wave - 2, gnext);
         }
         __syncthreads();
-        const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p);
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p.DK, p.DV);
         float qd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < KPW; ++w) {
@@ -781,8 +931,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             }
         }
     }
-    if (p.dstate0) {
-        const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.dstate0 + bh * sst, p);
+    if (seg == 0 && p.dstate0) {
+        const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.dstate0 + bh * sst, p.DK, p.DV);
 #pragma unroll
         for (int w = 0; w < TPW; ++w)
             if (wave + w * NW < DVT) {
@@ -829,7 +979,7 @@ __global__ __launch_bounds__(256) void delta_step_k(const Seq p, int slices) {
     const E* k = reinterpret_cast<const E*>(p.k) + b * p.sk[1] + hk * p.sk[2];
     const E* v = reinterpret_cast<const E*>(p.v) + b * p.sv[1] + h * p.sv[2] + (mine ? col : 0);
     const long long sst = (long long)p.DK * p.DV;
-    const __amdgpu_buffer_rsrc_t r0 = state_rsrc(p.state0 + bh * sst, p), r1 = state_rsrc(p.state_out + bh * sst, p);
+    const __amdgpu_buffer_rsrc_t r0 = state_rsrc(p.state0 + bh * sst, p.DK, p.DV), r1 = state_rsrc(p.state_out + bh * sst, p.DK, p.DV);
     const unsigned off = mine ? 4u * (grp * p.DV + col) : kOutside, srow = 16u * p.DV;     // row 4 i + grp: off + i * srow
     float S[R][VEC];
 #pragma unroll
@@ -911,6 +1061,28 @@ const char* sizes_error(const dcc_delta_seq* s) {
 bool rows_vec(const void* p, const long long* st, int dim, int dtype) {
     return aligned(p, 4 * esize(dtype)) && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0 && dim % 4 == 0;
 }
+// Segments of a call whose workgroups (row, head and, forward, 64 value columns) leave most of the chip idle: enough to fill it, none
+// shorter than 16 chunks.  The summaries cost about what the pass itself does, so a chip that is half full is left alone.
+int segments_of(const dcc_delta_seq* s, bool backward, int& seglen) {
+    const int64_t nchunk = (s->T + kC - 1) / kC, wgs = s->B * s->H * (backward ? 1 : (s->DV + 63) / 64);
+    int64_t n = 1;
+    if (wgs > 0 && wgs <= kSegBelow) n = std::max<int64_t>(1, std::min<int64_t>(kSegFill / wgs, nchunk / kSegMin));
+    int64_t len = (nchunk + n - 1) / n;
+    len = (len + 3) / 4 * 4;            // whole blocks
+    seglen = (int)std::max<int64_t>(len, 4);
+    return (int)std::max<int64_t>(1, (nchunk + seglen - 1) / seglen);
+}
+int64_t segment_floats(const dcc_delta_seq* s, int nseg) {
+    if (nseg <= 1) return 0;
+    return s->B * s->H * ((int64_t)(nseg - 1) * s->DK * (s->DV + s->DK) + (int64_t)nseg * s->DK * s->DV);
+}
+void place_segments(Seq& p, float* ws) {
+    if (p.nseg <= 1) return;
+    const int64_t bh = p.B * p.H;
+    p.sumN = ws;
+    p.sumP = p.sumN + bh * (p.nseg - 1) * p.DK * p.DV;
+    p.segS = p.sumP + bh * (p.nseg - 1) * p.DK * p.DK;
+}
 Seq base(const dcc_delta_seq* s) {
     Seq p = {};
     p.T = s->T; p.B = s->B; p.HK = s->HK; p.H = s->H; p.DK = s->DK; p.DV = s->DV; p.rep = s->H / s->HK;
@@ -935,20 +1107,31 @@ bool allow_lds(K kernel, size_t bytes) {
     return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
 }
 
-template <typename E, int DKT, int BT, int NW, bool VEC>
-int launch_fwd(const Seq& p, hipStream_t st) {
-    constexpr int KP = DKT * 16 + 4;
-    const size_t lds = sizeof(float) * (2 * BT * kC * KP + 2 * BT * kC * kSP) + BT * sizeof(ChunkVec);
-    const int nt = (p.DV + 15) / 16;
-    if (!allow_lds(delta_fwd_k<E, DKT, BT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_fwd: shared memory refused");
-    hipLaunchKernelGGL((delta_fwd_k<E, DKT, BT, NW, VEC>), dim3((unsigned)(p.B * p.H), (nt + NW - 1) / NW), dim3(64 * NW), lds, st, p);
-    return done("dcc_delta_fwd");
+template <typename E, int DKT, int BT, int NW, bool VEC, int MODE>
+int launch_walk(const Seq& p, hipStream_t st) {
+    constexpr int KP = DKT * 16 + 4, TILES = MODE == SUM_FWD ? 1 : 2;
+    const size_t lds = sizeof(float) * TILES * (BT * kC * KP + BT * kC * kSP) + BT * sizeof(ChunkVec);
+    const int nt = (p.DV + 15) / 16 + (MODE == FULL ? 0 : (p.DK + 15) / 16);
+    if (!allow_lds(delta_fwd_k<E, DKT, BT, NW, VEC, MODE>, lds)) return dcc_fail(kEHIP, "gated delta rule: shared memory refused");
+    hipLaunchKernelGGL((delta_fwd_k<E, DKT, BT, NW, VEC, MODE>), dim3((unsigned)(p.B * p.H), (nt + NW - 1) / NW, MODE == FULL ? p.nseg : p.nseg - 1),
+                       dim3(64 * NW), lds, st, p);
+    return done("gated delta rule");
+}
+// segment summaries and the states at the segments' starts (dir SUM_FWD) or ends (SUM_BWD)
+template <typename E, int DKT, int DIR>
+int segments(const Seq& p, hipStream_t st) {
+    const int rc = p.vec ? launch_walk<E, DKT, 4, 4, true, DIR>(p, st) : launch_walk<E, DKT, 1, 4, false, DIR>(p, st);
+    if (rc != 0) return rc;
+    hipLaunchKernelGGL((delta_join_k<DKT>), dim3((unsigned)(p.B * p.H), (p.DV + 15) / 16), dim3(64 * DKT), 0, st, p, DIR == SUM_BWD);
+    return done("gated delta rule");
 }
 template <typename E, int DKT>
 int fwd_dk(const Seq& p, hipStream_t st) {
-    if (!p.vec) return launch_fwd<E, DKT, 1, 4, false>(p, st);
-    if (p.nchunk <= 1) return p.DV <= 32 ? launch_fwd<E, DKT, 1, 2, true>(p, st) : launch_fwd<E, DKT, 1, 4, true>(p, st);
-    return p.DV <= 32 ? launch_fwd<E, DKT, 2, 2, true>(p, st) : launch_fwd<E, DKT, 4, 4, true>(p, st);
+    if (p.nseg > 1)
+        if (const int rc = segments<E, DKT, SUM_FWD>(p, st)) return rc;
+    if (!p.vec) return launch_walk<E, DKT, 1, 4, false, FULL>(p, st);
+    if (p.nchunk <= 1) return p.DV <= 32 ? launch_walk<E, DKT, 1, 2, true, FULL>(p, st) : launch_walk<E, DKT, 1, 4, true, FULL>(p, st);
+    return p.DV <= 32 ? launch_walk<E, DKT, 2, 2, true, FULL>(p, st) : launch_walk<E, DKT, 4, 4, true, FULL>(p, st);
 }
 template <typename E>
 int fwd_typed(const Seq& p, hipStream_t st) {
@@ -961,13 +1144,15 @@ int launch_bwd(const Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, VP = DVT * 16 + 4;
     const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 6 * NW * 16 + 2 * NW) + 2 * sizeof(ChunkTiles);
     if (!allow_lds(delta_bwd_k<E, DKT, DVT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_bwd: shared memory refused");
-    hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3((unsigned)(p.B * p.H)), dim3(64 * NW), lds, st, p);
+    hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3((unsigned)(p.B * p.H), p.nseg), dim3(64 * NW), lds, st, p);
     return done("dcc_delta_bwd");
 }
 template <typename E, int DKT>
 int bwd_dv(const Seq& p, hipStream_t st) {
     const int t = (p.DV + 15) / 16;
     constexpr int NW = DKT > 4 ? 8 : 4;
+    if (p.nseg > 1)
+        if (const int rc = segments<E, DKT, SUM_BWD>(p, st)) return rc;
     if (!p.vec) return launch_bwd<E, DKT, 8, 8, false>(p, st);
     return t <= 2 ? launch_bwd<E, DKT, 2, NW, true>(p, st) : t <= 4 ? launch_bwd<E, DKT, 4, NW, true>(p, st) : launch_bwd<E, DKT, 8, 8, true>(p, st);
 }
@@ -1006,18 +1191,24 @@ DCC_API int64_t dcc_delta_ckpt_floats(const dcc_delta_seq* s) {
     if (sizes_error(s)) return 0;
     return s->B * s->H * ((s->T + kC - 1) / kC + 1) * (int64_t)s->DK * s->DV;
 }
-DCC_API int64_t dcc_delta_fwd_workspace_floats(const dcc_delta_seq* s) { (void)s; return 0; }
+DCC_API int64_t dcc_delta_fwd_workspace_floats(const dcc_delta_seq* s) {
+    int len;
+    return sizes_error(s) ? 0 : segment_floats(s, segments_of(s, false, len));
+}
 DCC_API int64_t dcc_delta_bwd_workspace_floats(const dcc_delta_seq* s) {
-    if (sizes_error(s) || s->H == s->HK) return 0;
-    return 2 * s->T * s->B * s->H * (int64_t)s->DK;
+    int len;
+    if (sizes_error(s)) return 0;
+    return segment_floats(s, segments_of(s, true, len)) + (s->H == s->HK ? 0 : 2 * s->T * s->B * s->H * (int64_t)s->DK);
 }
 
 DCC_API int dcc_delta_fwd(const dcc_delta_seq* s, float* workspace, void* stream) {
-    (void)workspace;
     if (const char* e = sizes_error(s)) return refuse("dcc_delta_fwd", e);
     if (s->B == 0) return 0;
     if (s->T > 0 && (!s->q || !s->k || !s->v || !s->g || !s->beta || !s->o)) return refuse("dcc_delta_fwd", "null pointer");
-    const Seq p = base(s);
+    if (dcc_delta_fwd_workspace_floats(s) > 0 && !workspace) return refuse("dcc_delta_fwd", "null workspace");
+    Seq p = base(s);
+    p.nseg = segments_of(s, false, p.seglen);
+    place_segments(p, workspace);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     switch (s->dtype) {
         case DCC_DELTA_F32: return fwd_typed<float>(p, st);
@@ -1036,9 +1227,13 @@ DCC_API int dcc_delta_bwd(const dcc_delta_seq* s, const dcc_delta_grad* d, float
     Seq p = base(s);
     if (dcc_delta_bwd_workspace_floats(s) > 0) {
         if (!workspace) return refuse("dcc_delta_bwd", "null workspace");
-        p.dq32 = workspace;
-        p.dk32 = workspace + s->T * s->B * s->H * (int64_t)s->DK;
+        if (s->H != s->HK) {
+            p.dq32 = workspace + segment_floats(s, segments_of(s, true, p.seglen));
+            p.dk32 = p.dq32 + s->T * s->B * s->H * (int64_t)s->DK;
+        }
     }
+    p.nseg = segments_of(s, true, p.seglen);
+    place_segments(p, workspace);
     p.dout = d->dout; p.dstate1 = d->dstate1; p.ckpt = const_cast<float*>(d->ckpt);
     for (int i = 0; i < 3; ++i) p.sdo[i] = d->st_do[i];
     p.dq = d->dq; p.dk = d->dk; p.dv = d->dv; p.dg = d->dg; p.dbeta = d->dbeta; p.dstate0 = d->dstate0;

@@ -170,6 +170,50 @@ def test_sequence_and_gradient(size, dtype):
         check(x, r["d" + n], T, DK, True, "d" + n)
 
 
+LONG = [(700, 1, 1, 2, 64, 64), (1000, 2, 2, 4, 33, 17), (1100, 1, 1, 1, 128, 128), (2100, 1, 1, 3, 16, 40), (1540, 2, 1, 2, 96, 20), (520, 3, 1, 1, 64, 96)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", LONG, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype,reset", [(torch.float32, 0.0), (torch.float32, 0.01), (torch.bfloat16, 0.002)])
+def test_long_sequences(size, dtype, reset):
+    """few rows and many tokens: the segments that run side by side are joined to the sequence's own result and gradient"""
+    T, B, HK, H, DK, DV = size
+    d = make(*size, dtype=dtype, reset=reset, seed=T + DK, device="cuda")
+    d["g"].mul_(0.05)                       # a long memory: states reach across segments
+    for n in NAMES:
+        d[n].requires_grad_(True)
+    gen = torch.Generator().manual_seed(9)
+    do = torch.randn(T, B, H, DV, generator=gen).to(dtype).cuda()
+    ds = torch.randn(B, H, DK, DV, generator=gen).cuda()
+    o, S = fused.gated_delta(*[d[n] for n in NAMES], d["masks"])
+    grads = torch.autograd.grad([o, S], [d[n] for n in NAMES], [do, ds])
+    r = reference(d, DK ** -0.5, do, ds, grads=True)
+    check(o, r["o"], T, DK, what="o")
+    check(S, r["last"], T, DK, what="last")
+    for n, x in zip(NAMES, grads):
+        check(x, r["d" + n], T, DK, True, "d" + n)
+
+
+@pytest.mark.gpu
+def test_a_restart_wipes_nan_across_segments():
+    """1600 tokens of one row: a NaN at token 40, a restart at 700 -- everything from there on equals the clean run, as do its gradients"""
+    size = T, B, HK, H, DK, DV = 1600, 1, 1, 2, 32, 32
+    d = make(*size, reset=0.0, seed=13, device="cuda")
+    d["masks"][700] = 0
+    outs = []
+    for dirty in (False, True):
+        x = {n: t.clone() for n, t in d.items()}
+        if dirty:
+            x["v"][40] = float("nan")
+        leaves = [x[n].requires_grad_(True) for n in NAMES]
+        o, S = fused.gated_delta(*leaves, x["masks"])
+        g = torch.autograd.grad([o[704:].sum() + S.sum()], leaves)
+        outs.append([o[704:], S] + [y[704:] for y in g[:5]])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("masked,state,dlast", list(itertools.product([False, True], repeat=3)))
 def test_optional_operands(masked, state, dlast):
