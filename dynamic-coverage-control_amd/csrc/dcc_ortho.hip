@@ -5,11 +5,13 @@
 //    m x m matrices, and X <- Q X at the end: two passes over X instead of two per step.  An error of A along a direction of small
 //    singular value grows by a^2 = 12 per step, so this side runs in float64 (fp64 MFMA): measured against float64 throughout, five steps
 //    of 256 x 2704 are 4e-7 off, where float32 steps are 5e-6 off (and float32 on this side 1e-4).  A group holds at most five steps.
-//    All its matrices are polynomials of one symmetric matrix: only lower tiles are computed, and mirrored.
+//    All its matrices are polynomials of one symmetric matrix: only lower tiles are computed, and mirrored.  |X|_F^2 is the trace of
+//    the unscaled A, so nothing else reads X before the end.
 //  * step by step (large and nearly square, where the float64 products would take longer): A = X X^T, B = a I + b A + c A^2, X <- B X.
-// Products over X are C = A B^T to 32 bits.  fp32 MFMA has 1/16 of the bf16 rate, so the operands are split into three bf16 parts
-// (x = hi + mid + lo exactly: 8 + 8 + 8 significant bits) while they are staged, and six bf16 products (hh, hm, mh, hl, lh, mm) are
-// accumulated in float32; what is dropped is below 2^-23 of a product.
+// Large products over X are C = A B^T of bf16 planes: fp32 MFMA has 1/16 of the bf16 rate, so a value is kept as the sum of bf16 parts
+// and the products of the parts are accumulated in float32.  float32 and float16 matrices take three parts (x = hi + mid + lo exactly:
+// 8 + 8 + 8 significant bits) and the six products hh, hm, mh, hl, lh, mm; what is dropped is below 2^-23 of a product.  bfloat16 matrices
+// take two parts and hh, hm, mh (2^-16 of a product: 1/64 of the half step that the result is rounded by).
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -28,137 +30,24 @@ namespace {
 
 constexpr int kEINVAL = -1, kEHIP = -2;
 constexpr int kMaxProds = 20;           // products per launch (their descriptions travel as kernel arguments)
-constexpr int kNormBlocks = 64;         // partial sums of a matrix's norm, at most
-constexpr int kBK = 32;                 // depth of one staged slice
+constexpr int kNormBlocks = 256;        // partial sums of a matrix's norm, at most
+constexpr int kBK = 32;                 // depth of one staged slice of a plane product
+constexpr int kTile = 128;              // its tile; planes are padded to it with zeros
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef double d4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef unsigned short ushort_t;
 
-struct Prod {                           // out = alpha * A B^T + beta * E + diag * I
-    const void *a, *b;
-    const float* e;
-    void* out;
-    const double* norm;                 // operands marked raw are divided by sqrt(sum of these) + eps
-    long long lda, ldb, ldo;
-    int rows, cols, K;
-    int dta, dtb, dto;                  // 0 f32, 1 bf16, 2 f16
-    int amode, bmode;                   // 0: (i, k) at i * ld + k;  1: at k * ld + i
-    int rawa, rawb, nnorm;
-    int sym, tcols;
-    float alpha, beta, diag;
-    int first;                          // first block of this product
-};
-struct Batch { Prod p[kMaxProds]; int n; float eps; };
-
-struct NormMat { const void* x; double* out; long long n; int blocks, first; };
-struct NormBatch { NormMat m[kMaxProds * 2]; int n, dtype; };
-
-__device__ __forceinline__ float load1(const void* p, long long i, int dt) {
-    if (dt == 0) return reinterpret_cast<const float*>(p)[i];
-    if (dt == 1) return __uint_as_float((unsigned)reinterpret_cast<const unsigned short*>(p)[i] << 16);
-    return __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
+__device__ __forceinline__ float get(float x) { return x; }
+__device__ __forceinline__ float get(__hip_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float get(__half x) { return __half2float(x); }
 __device__ __forceinline__ void store1(void* p, long long i, int dt, float v) {
     if (dt == 0) reinterpret_cast<float*>(p)[i] = v;
     else if (dt == 1) reinterpret_cast<__hip_bfloat16*>(p)[i] = __float2bfloat16(v);
     else reinterpret_cast<__half*>(p)[i] = __float2half(v);
 }
-
-// sum of squares in float64, kNormBlocks fixed ranges per matrix
-__global__ __launch_bounds__(256) void ortho_norm_k(const NormBatch nb) {
-    __shared__ double red[4];
-    int i = 0;
-    while (i + 1 < nb.n && (int)blockIdx.x >= nb.m[i + 1].first) ++i;
-    const NormMat& m = nb.m[i];
-    const int blk = blockIdx.x - m.first;
-    const long long per = ((m.n + m.blocks - 1) / m.blocks + 3) & ~3ll;
-    const long long lo = blk * per, hi = lo + per < m.n ? lo + per : m.n;
-    double s0 = 0., s1 = 0., s2 = 0., s3 = 0.;
-    const long long hi4 = lo + ((hi > lo ? hi - lo : 0) & ~3ll);
-    const bool v4 = nb.dtype == 0 && (reinterpret_cast<uintptr_t>(m.x) & 15) == 0;
-    for (long long j = lo + 4 * threadIdx.x; j < hi4; j += 1024) {
-        float4 x;
-        if (v4) x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(m.x) + j);
-        else x = make_float4(load1(m.x, j, nb.dtype), load1(m.x, j + 1, nb.dtype), load1(m.x, j + 2, nb.dtype), load1(m.x, j + 3, nb.dtype));
-        s0 += (double)x.x * x.x; s1 += (double)x.y * x.y; s2 += (double)x.z * x.z; s3 += (double)x.w * x.w;
-    }
-    if (hi4 + threadIdx.x < hi) { const double x = load1(m.x, hi4 + threadIdx.x, nb.dtype); s0 += x * x; }
-    double s = (s0 + s1) + (s2 + s3);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) m.out[blk] = (red[0] + red[1]) + (red[2] + red[3]);
-}
-
-__device__ __forceinline__ float inverse_norm(const Prod& p, float eps) {
-    double s = 0.;
-    for (int i = 0; i < p.nnorm; ++i) s += p.norm[i];
-    return (float)(1.0 / (sqrt(s) + (double)eps));
-}
-
-// eight values of row i at depth k (zero outside); consecutive in memory for mode 0
-__device__ __forceinline__ void fetch8(float (&x)[8], const void* base, int dt, long long ld, int mode, int i, int rows, int k, int kend, bool vec) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    if (i >= rows) return;
-    if (mode == 0) {
-        const long long at = (long long)i * ld + k;
-        if (vec && k + 7 < kend) {
-            if (dt == 0) {
-                const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
-                const float4 a = p[0], b = p[1];
-                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-            } else {
-                const u4 a = *reinterpret_cast<const u4*>(reinterpret_cast<const unsigned short*>(base) + at);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (dt == 1) {
-                        x[2 * j] = __uint_as_float(a[j] << 16);
-                        x[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
-                    } else {
-                        const unsigned w = a[j];
-                        const __half2 h = *reinterpret_cast<const __half2*>(&w);
-                        x[2 * j] = __low2float(h);
-                        x[2 * j + 1] = __high2float(h);
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k + j < kend) x[j] = load1(base, at + j, dt);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (k + j < kend) x[j] = load1(base, (long long)(k + j) * ld + i, dt);
-    }
-}
-
-// x * s split into three bf16 parts by truncation: exact, every part has at most 8 significant bits
-__device__ __forceinline__ void split8(const float (&x)[8], float s, u4& hi, u4& mid, u4& lo) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        unsigned h[2], m[2], l[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float v = x[2 * j + e] * s;
-            h[e] = __float_as_uint(v) & 0xffff0000u;
-            const float r = v - __uint_as_float(h[e]);
-            m[e] = __float_as_uint(r) & 0xffff0000u;
-            l[e] = __float_as_uint(r - __uint_as_float(m[e]));
-        }
-        hi[j] = (h[0] >> 16) | h[1];
-        mid[j] = (m[0] >> 16) | m[1];
-        lo[j] = (l[0] >> 16) | (l[1] & 0xffff0000u);
-    }
-}
-
-// 16-byte piece kg of row i in a staged plane: the pieces of a row are turned by i / 4, so that the 16 rows that one MFMA operand
-// reads at one kg lie in 16 different groups of banks
-__device__ __forceinline__ int piece(int i, int kg) { return i * 4 + (kg ^ ((i >> 2) & 3)); }
 
 // tile (ti, tj), tj <= ti, of the lower triangle counted row by row
 __device__ __forceinline__ void lower_tile(int blk, int& ti, int& tj) {
@@ -168,176 +57,100 @@ __device__ __forceinline__ void lower_tile(int blk, int& ti, int& tj) {
     tj = blk - ti * (ti + 1) / 2;
 }
 
-// One workgroup: one TM x TM tile of one product (4 waves as 2 x 2).
-template <int TM>
-__global__ __launch_bounds__(256) void ortho_prod_k(const Batch bt) {
-    constexpr int TW = TM / 2, NT = TW / 16, PASS = TM / 64;
-    __shared__ u4 sh[2 * 3 * TM * 4];
-    int pi = 0;
-    while (pi + 1 < bt.n && (int)blockIdx.x >= bt.p[pi + 1].first) ++pi;
-    const Prod& p = bt.p[pi];
-    int blk = blockIdx.x - p.first;
-    int ti, tj;
-    if (p.sym) {
-        lower_tile(blk, ti, tj);
-    } else {
-        ti = blk / p.tcols;
-        tj = blk - ti * p.tcols;
-    }
-    const int i0 = ti * TM, j0 = tj * TM;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 15, kg = lane >> 4, g4 = kg << 2;
-    const int wi = (wave >> 1) * TW, wj = (wave & 1) * TW;
-    const float inv = (p.rawa | p.rawb) ? inverse_norm(p, bt.eps) : 1.f;
-    const float sa = p.rawa ? inv : 1.f, sb = p.rawb ? inv : 1.f;
-    const bool va = p.amode == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0 && p.lda % 8 == 0;
-    const bool vb = p.bmode == 0 && (reinterpret_cast<uintptr_t>(p.b) & 15) == 0 && p.ldb % 8 == 0;
-    const int ra = p.amode == 0 ? tid >> 2 : tid & 63, ka = p.amode == 0 ? tid & 3 : tid >> 6;
-    const int rb = p.bmode == 0 ? tid >> 2 : tid & 63, kb = p.bmode == 0 ? tid & 3 : tid >> 6;
-    const int kend = p.K;
+// Where |X|_F^2 comes from: `n` numbers at stride `step` (the diagonal of X X^T, or partial sums).  Every workgroup that needs it sums
+// them for itself, in one order.  A null pointer: X is scaled already.
+struct Scale { const double* at; long long step; int n; float eps; };
+__device__ __forceinline__ double inverse_norm(const Scale& s, double* red, double* note = nullptr) {    // red: 4 doubles of LDS; all 256 threads
+    if (!s.at) return 1.;
+    double v = 0.;
+    for (int i = threadIdx.x; i < s.n; i += 256) v += s.at[i * s.step];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (red[0] + red[1]) + (red[2] + red[3]);
+    if (note && threadIdx.x == 0) *note = v;
+    return 1. / (sqrt(v) + (double)s.eps);
+}
 
-    f4 acc[NT][NT];
+struct NormMat { const void* x; double* out; long long n; int blocks, first; };
+struct NormBatch { NormMat m[2 * kMaxProds]; int n; };
+
+// sum of squares in float64, by fixed ranges
+template <typename E>
+__global__ __launch_bounds__(256) void ortho_norm_k(const NormBatch nb) {
+    __shared__ double red[4];
+    int i = 0;
+    while (i + 1 < nb.n && (int)blockIdx.x >= nb.m[i + 1].first) ++i;
+    const NormMat& m = nb.m[i];
+    const E* x = reinterpret_cast<const E*>(m.x);
+    const int blk = blockIdx.x - m.first;
+    const long long per = (m.n + m.blocks - 1) / m.blocks, lo = blk * per, hi = lo + per < m.n ? lo + per : m.n;
+    double s[4] = {0., 0., 0., 0.};
+    long long j = lo + threadIdx.x;
+    for (; j + 768 < hi; j += 1024)
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+        for (int e = 0; e < 4; ++e) { const double v = get(x[j + 256 * e]); s[e] += v * v; }
+    for (; j < hi; j += 256) { const double v = get(x[j]); s[0] += v * v; }
+    double t = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
-        for (int y = 0; y < NT; ++y) acc[x][y] = f4{0.f, 0.f, 0.f, 0.f};
-    float xa[PASS][8], xb[PASS][8];
-#pragma unroll
-    for (int q = 0; q < PASS; ++q) {
-        fetch8(xa[q], p.a, p.dta, p.lda, p.amode, i0 + q * 64 + ra, p.rows, ka * 8, kend, va);
-        fetch8(xb[q], p.b, p.dtb, p.ldb, p.bmode, j0 + q * 64 + rb, p.cols, kb * 8, kend, vb);
-    }
-    for (int k = 0; k < kend; k += kBK) {
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < PASS; ++q) {
-            u4 h, m, l;
-            split8(xa[q], sa, h, m, l);
-            const int pa = piece(q * 64 + ra, ka), pb = piece(q * 64 + rb, kb);
-            sh[pa] = h; sh[TM * 4 + pa] = m; sh[2 * TM * 4 + pa] = l;
-            split8(xb[q], sb, h, m, l);
-            sh[3 * TM * 4 + pb] = h; sh[4 * TM * 4 + pb] = m; sh[5 * TM * 4 + pb] = l;
-        }
-        __syncthreads();
-        if (k + kBK < kend) {
-#pragma unroll
-            for (int q = 0; q < PASS; ++q) {
-                fetch8(xa[q], p.a, p.dta, p.lda, p.amode, i0 + q * 64 + ra, p.rows, k + kBK + ka * 8, kend, va);
-                fetch8(xb[q], p.b, p.dtb, p.ldb, p.bmode, j0 + q * 64 + rb, p.cols, k + kBK + kb * 8, kend, vb);
-            }
-        }
-        bf8 fb[NT][3];
-#pragma unroll
-        for (int y = 0; y < NT; ++y) {
-            const int pb = piece(wj + 16 * y + li, kg);
-#pragma unroll
-            for (int s = 0; s < 3; ++s) fb[y][s] = __builtin_bit_cast(bf8, sh[(3 + s) * TM * 4 + pb]);
-        }
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-            const int pa = piece(wi + 16 * x + li, kg);
-            bf8 fa[3];
-#pragma unroll
-            for (int s = 0; s < 3; ++s) fa[s] = __builtin_bit_cast(bf8, sh[s * TM * 4 + pa]);
-#pragma unroll
-            for (int y = 0; y < NT; ++y) {
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[0], fb[y][2], acc[x][y], 0, 0, 0);
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[2], fb[y][0], acc[x][y], 0, 0, 0);
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[1], fb[y][1], acc[x][y], 0, 0, 0);
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[0], fb[y][1], acc[x][y], 0, 0, 0);
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[1], fb[y][0], acc[x][y], 0, 0, 0);
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[0], fb[y][0], acc[x][y], 0, 0, 0);
-            }
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int y = 0; y < NT; ++y)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = i0 + wi + 16 * x + g4 + r, j = j0 + wj + 16 * y + li;
-                if (i >= p.rows || j >= p.cols) continue;
-                if (p.sym && j > i) continue;               // its mirror is written below
-                float v = p.alpha * acc[x][y][r];
-                if (p.e) v += p.beta * p.e[(long long)i * p.cols + j];
-                if (i == j) v += p.diag;
-                store1(p.out, (long long)i * p.ldo + j, p.dto, v);
-                if (p.sym && i != j) store1(p.out, (long long)j * p.ldo + i, p.dto, v);
-            }
+    for (int o = 32; o >= 1; o >>= 1) t += __shfl_xor(t, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) m.out[blk] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // ---- the m x m side in float64 -------------------------------------------------------------------------------------------------
-struct DProd {                          // out = alpha * A B^T + beta * E + diag * I, symmetric, m x m
-    const void *a, *b;
-    const double* e;
-    void* out;
-    double* part;                       // slices > 1: partial sums [slices][m * m]
-    const double* norm;                 // raw operands: the result is divided by (sqrt(sum of these) + eps)^2
-    long long lda, ldb;
-    int m, K, dt, mode, nnorm, slices, kper, out32, first;      // dt: 0 f32, 1 bf16, 2 f16, 3 f64; mode as above (f64: 0)
-    double alpha, beta, diag;
+// v_mfma_f64_16x16x4_f64: A[i = lane%16][k = lane/16], B[k = lane/16][j = lane%16], D[i = 4 r + lane/16][j = lane%16]; a lane's four
+// consecutive k make four steps.  Square matrices are stored [mq][mq], mq = m rounded up to 16, zero outside m: no bounds to check.
+struct Gram {                           // out = X X^T, X [m, K] in memory as [m][K] or, tall, [K][m]
+    const void* x;
+    double *out, *part;                 // part: [slices][mq * mq] where slices > 1
+    long long ld;
+    int m, mq, K, slices, kper, first;  // kper: a multiple of 16
 };
-struct DBatch { DProd p[kMaxProds]; int n; float eps; };
-typedef double d4 __attribute__((ext_vector_type(4)));
+struct GramBatch { Gram p[kMaxProds]; int n; };
 
-// four values of row i at depth k, zero outside
-__device__ __forceinline__ d4 fetch4(const void* base, int dt, long long ld, int mode, int i, int rows, int k, int kend, bool vec) {
-    d4 x = {0., 0., 0., 0.};
-    if (i >= rows) return x;
-    const long long at = mode == 0 ? (long long)i * ld + k : (long long)k * ld + i, step = mode == 0 ? 1 : ld;
-    if (dt == 3) {
-        const double* p = reinterpret_cast<const double*>(base) + at;
-        if (vec && k + 3 < kend) {
-            const double2 u = reinterpret_cast<const double2*>(p)[0], w = reinterpret_cast<const double2*>(p)[1];
-            x[0] = u.x; x[1] = u.y; x[2] = w.x; x[3] = w.y;
-        } else {
+// four values of row i (< m, or cleared) at depth k
+template <typename E, bool TALL, bool VEC>
+__device__ __forceinline__ d4 fetch_x(const E* x, long long ld, int i, int m, int k, int kend) {
+    d4 v;
+    const int ic = i < m ? i : m - 1;
+    if constexpr (VEC) {
+        struct alignas(4 * sizeof(E)) Four { E e[4]; };
+        const Four f = *reinterpret_cast<const Four*>(x + (long long)ic * ld + (k < kend ? k : 0));
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (k + j < kend) x[j] = p[j];
+        for (int j = 0; j < 4; ++j) v[j] = i < m && k < kend ? (double)get(f.e[j]) : 0.;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int kc = k + j < kend ? k + j : kend - 1;
+            const float f = get(TALL ? x[(long long)kc * ld + ic] : x[(long long)ic * ld + kc]);
+            v[j] = i < m && k + j < kend ? (double)f : 0.;
         }
-    } else if (vec && dt == 0 && k + 3 < kend) {
-        const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (k + j < kend) x[j] = load1(base, at + j * step, dt);
     }
-    return x;
+    return v;
 }
 
-__device__ __forceinline__ void dstore(const DProd& p, const DBatch& bt, double v, int i, int j) {
-    if (p.nnorm > 0) {
-        double s = 0.;
-        for (int q = 0; q < p.nnorm; ++q) s += p.norm[q];
-        s = sqrt(s) + (double)bt.eps;
-        v /= s * s;
-    }
-    v *= p.alpha;
-    const long long ij = (long long)i * p.m + j, ji = (long long)j * p.m + i;
-    if (p.e) v += p.beta * p.e[ij];
-    if (i == j) v += p.diag;
-    if (p.out32) {
-        reinterpret_cast<float*>(p.out)[ij] = (float)v;
-        reinterpret_cast<float*>(p.out)[ji] = (float)v;
-    } else {
-        reinterpret_cast<double*>(p.out)[ij] = v;
-        reinterpret_cast<double*>(p.out)[ji] = v;
-    }
+__device__ __forceinline__ void mirror(double* out, int mq, int i, int j, double v) {
+    out[(long long)i * mq + j] = v;
+    out[(long long)j * mq + i] = v;
 }
 
-// v_mfma_f64_16x16x4_f64: A[i = lane%16][k = lane/16], B[k = lane/16][j = lane%16], D[i = 4 r + lane/16][j = lane%16].  Operands come from
-// memory as they are (a lane's four consecutive k make four steps).  WIDE: a 64 x 64 tile by 2 x 2 waves of 32 x 32 (long depths, where
-// reading the operands counts); else a 16 x 16 tile whose depth the four waves share (short ones, where latency does).
-template <bool WIDE>
-__global__ __launch_bounds__(256) void ortho_dprod_k(const DBatch bt) {
+// WIDE: a 64 x 64 tile by 2 x 2 waves of 32 x 32 (long depths, where reading the operands counts); else a 16 x 16 tile whose depth the
+// four waves share (short ones, where latency does).  VEC: rows of X may be read four elements at a time (K a multiple of 4).
+template <typename E, bool TALL, bool VEC, bool WIDE>
+__global__ __launch_bounds__(256) void ortho_gram_k(const GramBatch bt) {
     constexpr int T = WIDE ? 2 : 1, TM = WIDE ? 64 : 16;
     __shared__ double sh[WIDE ? 1 : 4 * 256];
     int pi = 0;
     while (pi + 1 < bt.n && (int)blockIdx.x >= bt.p[pi + 1].first) ++pi;
-    const DProd& p = bt.p[pi];
-    int blk = blockIdx.x - p.first, ti, tj;
-    const int slice = blk % p.slices;
+    const Gram& p = bt.p[pi];
+    const E* x = reinterpret_cast<const E*>(p.x);
+    const int blk = blockIdx.x - p.first, slice = blk % p.slices, m = p.m, mq = p.mq;
+    const long long ld = p.ld;
+    int ti, tj;
     lower_tile(blk / p.slices, ti, tj);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
     const int i0 = ti * TM + (WIDE ? (wave >> 1) * 32 : 0), j0 = tj * TM + (WIDE ? (wave & 1) * 32 : 0);
@@ -347,26 +160,35 @@ __global__ __launch_bounds__(256) void ortho_dprod_k(const DBatch bt) {
         kbeg += wave * quarter;
         kend = kbeg + quarter < kend ? kbeg + quarter : kend;
     }
-    const bool va = p.mode == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0 && p.lda % 4 == 0;
-    const bool vb = p.mode == 0 && (reinterpret_cast<uintptr_t>(p.b) & 15) == 0 && p.ldb % 4 == 0;
     d4 acc[T][T];
 #pragma unroll
-    for (int x = 0; x < T; ++x)
+    for (int a = 0; a < T; ++a)
 #pragma unroll
-        for (int y = 0; y < T; ++y) acc[x][y] = d4{0., 0., 0., 0.};
-    for (int k = kbeg; k < kend; k += 16) {
-        d4 a[T], b[T];
+        for (int c = 0; c < T; ++c) acc[a][c] = d4{0., 0., 0., 0.};
+    if (kbeg < kend) {
+        d4 na[T], nb[T];
 #pragma unroll
-        for (int x = 0; x < T; ++x) {
-            a[x] = fetch4(p.a, p.dt, p.lda, p.mode, i0 + 16 * x + li, p.m, k + 4 * g, kend, va);
-            b[x] = fetch4(p.b, p.dt, p.ldb, p.mode, j0 + 16 * x + li, p.m, k + 4 * g, kend, vb);
+        for (int t = 0; t < T; ++t) {
+            na[t] = fetch_x<E, TALL, VEC>(x, ld, i0 + 16 * t + li, m, kbeg + 4 * g, kend);
+            nb[t] = fetch_x<E, TALL, VEC>(x, ld, j0 + 16 * t + li, m, kbeg + 4 * g, kend);
         }
+        for (int k = kbeg; k < kend; k += 16) {
+            d4 a[T], b[T];
 #pragma unroll
-        for (int x = 0; x < T; ++x)
+            for (int t = 0; t < T; ++t) { a[t] = na[t]; b[t] = nb[t]; }
+            const int kn = k + 16 < kend ? k + 16 : k;
 #pragma unroll
-            for (int y = 0; y < T; ++y)
+            for (int t = 0; t < T; ++t) {
+                na[t] = fetch_x<E, TALL, VEC>(x, ld, i0 + 16 * t + li, m, kn + 4 * g, kend);
+                nb[t] = fetch_x<E, TALL, VEC>(x, ld, j0 + 16 * t + li, m, kn + 4 * g, kend);
+            }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[x][y] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[x][r], b[y][r], acc[x][y], 0, 0, 0);
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int s = 0; s < T; ++s)
+#pragma unroll
+                    for (int c = 0; c < T; ++c) acc[s][c] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[s][r], b[c][r], acc[s][c], 0, 0, 0);
+        }
     }
     if (!WIDE) {
 #pragma unroll
@@ -374,35 +196,363 @@ __global__ __launch_bounds__(256) void ortho_dprod_k(const DBatch bt) {
         __syncthreads();
         const int i = i0 + (threadIdx.x >> 4), j = j0 + (threadIdx.x & 15);
         const double v = (sh[threadIdx.x] + sh[256 + threadIdx.x]) + (sh[512 + threadIdx.x] + sh[768 + threadIdx.x]);
-        if (i < p.m && j <= i) {
-            if (p.slices > 1) p.part[((long long)slice * p.m + i) * p.m + j] = v;
-            else dstore(p, bt, v, i, j);
+        if (j <= i) {
+            if (p.slices > 1) p.part[((long long)slice * mq + i) * mq + j] = v;
+            else mirror(p.out, mq, i, j, v);
         }
         return;
     }
 #pragma unroll
-    for (int x = 0; x < T; ++x)
+    for (int s = 0; s < T; ++s)
 #pragma unroll
-        for (int y = 0; y < T; ++y)
+        for (int c = 0; c < T; ++c)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = i0 + 16 * x + 4 * r + g, j = j0 + 16 * y + li;
-                if (i >= p.m || j > i) continue;
-                if (p.slices > 1) p.part[((long long)slice * p.m + i) * p.m + j] = acc[x][y][r];
-                else dstore(p, bt, acc[x][y][r], i, j);
+                const int i = i0 + 16 * s + 4 * r + g, j = j0 + 16 * c + li;
+                if (i >= mq || j > i) continue;
+                if (p.slices > 1) p.part[((long long)slice * mq + i) * mq + j] = acc[s][c][r];
+                else mirror(p.out, mq, i, j, acc[s][c][r]);
             }
 }
 
-__global__ __launch_bounds__(256) void ortho_djoin_k(const DBatch bt) {
-    const DProd& p = bt.p[blockIdx.y];
+__global__ __launch_bounds__(256) void ortho_join_k(const GramBatch bt) {
+    const Gram& p = bt.p[blockIdx.y];
     if (p.slices <= 1) return;
-    const long long n = (long long)p.m * p.m;
+    const long long n = (long long)p.mq * p.mq;
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
-        const int i = (int)(at / p.m), j = (int)(at - (long long)i * p.m);
+        const int i = (int)(at / p.mq), j = (int)(at - (long long)i * p.mq);
         if (j > i) continue;
         double s = 0.;
         for (int q = 0; q < p.slices; ++q) s += p.part[q * n + at];
-        dstore(p, bt, s, i, j);
+        mirror(p.out, p.mq, i, j, s);
+    }
+}
+
+// Three planes of a value (NP 2: two).  All but the last part are truncated, so that the parts add up to the value exactly while it has
+// bits left; the last is rounded to nearest.
+template <int NP>
+__device__ __forceinline__ void split(float v, ushort_t (&h)[NP]) {
+#pragma unroll
+    for (int s = 0; s + 1 < NP; ++s) {
+        const unsigned u = __float_as_uint(v) & 0xffff0000u;
+        h[s] = (ushort_t)(u >> 16);
+        v -= __uint_as_float(u);
+    }
+    const __hip_bfloat16 r = __float2bfloat16(v);
+    h[NP - 1] = __builtin_bit_cast(ushort_t, r);
+}
+
+struct Square {                         // out = alpha A B + beta E + diag I, all symmetric [mq][mq]; A is E of the unscaled matrix: see sa
+    const double *a, *b, *e;
+    double* out;                        // null: three planes instead, [mp][mp] of stride plane
+    ushort_t* planes;
+    long long plane;
+    int m, mq, mp, first;
+    double alpha, beta, diag;
+    Scale s;                            // beta (E) is scaled by 1 / norm^2, alpha by its power sa (twice for A A of the unscaled A)
+    int sa;
+    double* note;                       // the first workgroup leaves norm^2 here, or null
+};
+struct SquareBatch { Square p[kMaxProds]; int n; };
+
+__global__ __launch_bounds__(256) void ortho_square_k(const SquareBatch bt) {
+    __shared__ double sh[4 * 256], red[4];
+    int pi = 0;
+    while (pi + 1 < bt.n && (int)blockIdx.x >= bt.p[pi + 1].first) ++pi;
+    const Square& p = bt.p[pi];
+    int ti, tj;
+    lower_tile(blockIdx.x - p.first, ti, tj);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4, mq = p.mq;
+    const int i0 = ti * 16, j0 = tj * 16;
+    d4 acc0 = {0., 0., 0., 0.}, acc1 = acc0;
+    if (i0 < mq) {                      // (padded planes reach behind mq: zeros)
+        const int quarter = ((mq + 3) / 4 + 15) & ~15, kbeg = wave * quarter, kend = kbeg + quarter < mq ? kbeg + quarter : mq;
+        const double* pa = p.a + (long long)(i0 + li) * mq + 4 * g;
+        const double* pb = p.b + (long long)(j0 + li) * mq + 4 * g;
+        for (int k = kbeg; k < kend; k += 16) {
+            const d4 a = *reinterpret_cast<const d4*>(pa + k), b = *reinterpret_cast<const d4*>(pb + k);
+            acc0 = __builtin_amdgcn_mfma_f64_16x16x4f64(a[0], b[0], acc0, 0, 0, 0);
+            acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(a[1], b[1], acc1, 0, 0, 0);
+            acc0 = __builtin_amdgcn_mfma_f64_16x16x4f64(a[2], b[2], acc0, 0, 0, 0);
+            acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(a[3], b[3], acc1, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sh[wave * 256 + (4 * r + g) * 16 + li] = acc0[r] + acc1[r];
+    const double inv = inverse_norm(p.s, red, (int)blockIdx.x == p.first ? p.note : nullptr), inv2 = inv * inv;
+    __syncthreads();
+    const int i = i0 + (threadIdx.x >> 4), j = j0 + (threadIdx.x & 15);
+    double v = (sh[threadIdx.x] + sh[256 + threadIdx.x]) + (sh[512 + threadIdx.x] + sh[768 + threadIdx.x]);
+    v *= p.alpha * (p.sa > 1 ? inv2 * inv2 : p.sa > 0 ? inv2 : 1.);
+    if (j > i) return;
+    if (p.e && i < mq) v += p.beta * inv2 * p.e[(long long)i * mq + j];
+    if (i == j && i < p.m) v += p.diag;
+    if (p.out) {
+        mirror(p.out, mq, i, j, v);
+    } else {
+        // (rounded once, from 64 bits to the planes' 24)
+        const float hi = (float)v;
+        ushort_t h[3];
+        split<3>(hi, h);
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            p.planes[s * p.plane + (long long)i * p.mp + j] = h[s];
+            p.planes[s * p.plane + (long long)j * p.mp + i] = h[s];
+        }
+    }
+}
+
+// X <- Q X in float64, for products that are too small to split: a 16 x 16 tile per wave, operands straight from memory.
+struct Apply {                          // out [rows][cols] = Q X (wide: X [m][n]) or X Q (tall: X [n][m])
+    const void* x;
+    const double* q;
+    void* out;
+    long long ld;                       // of X and out
+    int m, mq, rows, cols, tcols, dto, first;
+    Scale s;
+};
+struct ApplyBatch { Apply p[kMaxProds]; int n; };
+
+template <typename E, bool TALL>
+__global__ __launch_bounds__(256) void ortho_apply_k(const ApplyBatch bt) {
+    __shared__ double red[4];
+    int pi = 0;
+    while (pi + 1 < bt.n && (int)blockIdx.x >= bt.p[pi + 1].first) ++pi;
+    const Apply& p = bt.p[pi];
+    const E* x = reinterpret_cast<const E*>(p.x);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4, m = p.m, mq = p.mq;
+    const long long ld = p.ld;
+    const double inv = inverse_norm(p.s, red);
+    const int tile = (blockIdx.x - p.first) * 4 + wave, ti = tile / p.tcols, tj = tile - ti * p.tcols, i0 = ti * 16, j0 = tj * 16;
+    if (i0 >= p.rows) return;
+    d4 acc0 = {0., 0., 0., 0.}, acc1 = acc0;
+    const double* pq = p.q + (long long)((TALL ? j0 : i0) + li) * mq + 4 * g;
+    const int row = TALL ? (i0 + li < p.rows ? i0 + li : p.rows - 1) : 0, c = TALL ? 0 : (j0 + li < p.cols ? j0 + li : p.cols - 1);
+    for (int k = 0; k < mq; k += 16) {
+        const d4 q = *reinterpret_cast<const d4*>(pq + k);
+        double v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int kk = k + 4 * g + r, kc = kk < m ? kk : m - 1;         // (Q is zero behind m)
+            v[r] = get(TALL ? x[(long long)row * ld + kc] : x[(long long)kc * ld + c]);
+        }
+        if (TALL) {
+            acc0 = __builtin_amdgcn_mfma_f64_16x16x4f64(v[0], q[0], acc0, 0, 0, 0);
+            acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(v[1], q[1], acc1, 0, 0, 0);
+            acc0 = __builtin_amdgcn_mfma_f64_16x16x4f64(v[2], q[2], acc0, 0, 0, 0);
+            acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(v[3], q[3], acc1, 0, 0, 0);
+        } else {
+            acc0 = __builtin_amdgcn_mfma_f64_16x16x4f64(q[0], v[0], acc0, 0, 0, 0);
+            acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(q[1], v[1], acc1, 0, 0, 0);
+            acc0 = __builtin_amdgcn_mfma_f64_16x16x4f64(q[2], v[2], acc0, 0, 0, 0);
+            acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64(q[3], v[3], acc1, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int i = i0 + 4 * r + g, j = j0 + li;
+        if (i < p.rows && j < p.cols) store1(p.out, (long long)i * ld + j, p.dto, (float)((acc0[r] + acc1[r]) * inv));
+    }
+}
+
+// ---- plane products ------------------------------------------------------------------------------------------------------------
+struct Split {                          // planes of the scaled X [R][C]: as it lies (`same` [rp][cp]) and / or transposed (`turned` [cp][rp])
+    const void* x;
+    ushort_t *same, *turned;
+    long long plane;                    // elements between planes
+    int R, C, rp, cp, tcols, first;     // padded to kTile with zeros
+    Scale s;
+};
+struct SplitBatch { Split p[kMaxProds]; int n; };
+
+template <typename E, int NP>
+__global__ __launch_bounds__(256) void ortho_split_k(const SplitBatch bt) {
+    __shared__ double red[4];
+    __shared__ alignas(16) ushort_t sh[NP][64][72];         // transposed tile: rows of 144 bytes
+    int pi = 0;
+    while (pi + 1 < bt.n && (int)blockIdx.x >= bt.p[pi + 1].first) ++pi;
+    const Split& p = bt.p[pi];
+    const E* x = reinterpret_cast<const E*>(p.x);
+    const int blk = blockIdx.x - p.first, i0 = blk / p.tcols * 64, j0 = blk % p.tcols * 64;
+    const float inv = (float)inverse_norm(p.s, red);
+    const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
+    const int jc = j0 + c < p.C ? j0 + c : p.C - 1;
+    float v[16];
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        const int i = i0 + r0 * 16 + q, ic = i < p.R ? i : p.R - 1;
+        v[q] = get(x[(long long)ic * p.C + jc]);
+        v[q] = i < p.R && j0 + c < p.C ? v[q] * inv : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+        ushort_t h[NP];
+        split<NP>(v[q], h);
+#pragma unroll
+        for (int s = 0; s < NP; ++s) {
+            if (p.same) p.same[s * p.plane + (long long)(i0 + r0 * 16 + q) * p.cp + j0 + c] = h[s];
+            if (p.turned) sh[s][c][r0 * 16 + q] = h[s];
+        }
+    }
+    if (!p.turned) return;
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < NP; ++s)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int e = threadIdx.x + q * 256, j = e >> 3, i = (e & 7) * 8;
+            *reinterpret_cast<u4*>(p.turned + s * p.plane + (long long)(j0 + j) * p.rp + i0 + i) = *reinterpret_cast<const u4*>(&sh[s][j][i]);
+        }
+}
+
+struct Gemm {                           // v = alpha A B^T + beta E + diag I
+    const ushort_t *a, *b, *e;          // planes; rows of A and B are contiguous over the depth
+    ushort_t *d1, *d2;                  // planes of v as [i][j] and as [j][i] (either may be null)
+    void* out;                          // or, bounded by rows and cols, v itself
+    long long pa, pb, pe, p1, p2, ldo;  // elements between planes; row length of out
+    int lda, ldb, lde, ld1, ld2, K, rows, cols, dto, sym, tcols, first;     // K: a multiple of kBK
+    float alpha, beta, diag;
+};
+struct GemmBatch { Gemm p[kMaxProds]; int n; };
+
+// 16-byte piece kg of row i in a staged slice: the pieces of a row are turned by i / 4, so that the 16 rows that one MFMA operand
+// reads at one kg lie in 16 different groups of banks
+__device__ __forceinline__ int piece(int i, int kg) { return i * 4 + (kg ^ ((i >> 2) & 3)); }
+
+// One 128 x 128 tile of one product: 4 waves as 2 x 2 of 64 x 64, slices of 32 in two stages that go to LDS directly.
+template <int NP>
+__global__ __launch_bounds__(256) void ortho_gemm_k(const GemmBatch bt) {
+    constexpr int kSlice = kTile * 4;                   // 16-byte pieces of one plane's slice
+    constexpr int kStage = 2 * NP * kSlice;
+    extern __shared__ u4 lds[];                         // [2][2 * NP][kSlice]
+    int pi = 0;
+    while (pi + 1 < bt.n && (int)blockIdx.x >= bt.p[pi + 1].first) ++pi;
+    const Gemm& p = bt.p[pi];
+    const int blk = blockIdx.x - p.first;
+    int ti, tj;
+    if (p.sym) {
+        lower_tile(blk, ti, tj);
+    } else {
+        ti = blk / p.tcols;
+        tj = blk - ti * p.tcols;
+    }
+    const int i0 = ti * kTile, j0 = tj * kTile;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, kg = lane >> 4, g4 = kg << 2;
+    const int wi = (wave >> 1) * 64, wj = (wave & 1) * 64;
+    // wave w brings rows 32 w .. 32 w + 31 of every plane, 16 at a time: lane l puts piece l % 4 of row l / 4
+    const int lrow = 32 * wave + (lane >> 2), lk = ((lane & 3) ^ ((lane >> 4) & 3)) * 8;
+    const ushort_t* ga = p.a + (long long)(i0 + lrow) * p.lda + lk;
+    const ushort_t* gb = p.b + (long long)(j0 + lrow) * p.ldb + lk;
+    const long long ra = 16ll * p.lda, rb = 16ll * p.ldb, pa = p.pa, pb = p.pb;
+    auto stage = [&](int which) {
+        u4* base = lds + which * kStage + wave * 128;
+#pragma unroll
+        for (int s = 0; s < NP; ++s)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(ga + s * pa + q * ra),
+                                                 (__attribute__((address_space(3))) void*)(base + s * kSlice + q * 64), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(gb + s * pb + q * rb),
+                                                 (__attribute__((address_space(3))) void*)(base + (NP + s) * kSlice + q * 64), 16, 0, 0);
+            }
+        ga += kBK;
+        gb += kBK;
+    };
+    f4 acc[4][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = f4{0.f, 0.f, 0.f, 0.f};
+    const int steps = p.K / kBK;
+    stage(0);
+    for (int k = 0; k < steps; ++k) {
+        if (k + 1 < steps) {
+            stage((k + 1) & 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * NP) : "memory");       // all but the 4 NP loads just issued
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __syncthreads();
+        const u4* sa = lds + (k & 1) * kStage;
+        const u4* sb = sa + NP * kSlice;
+        bf8 fb[4][NP];
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int s = 0; s < NP; ++s) fb[y][s] = __builtin_bit_cast(bf8, sb[s * kSlice + piece(wj + 16 * y + li, kg)]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            bf8 fa[NP];
+#pragma unroll
+            for (int s = 0; s < NP; ++s) fa[s] = __builtin_bit_cast(bf8, sa[s * kSlice + piece(wi + 16 * x + li, kg)]);
+            // small products first
+#pragma unroll
+            for (int o = NP - 1; o >= 0; --o)
+#pragma unroll
+                for (int s = 0; s <= o; ++s)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s], fb[y][o - s], acc[x][y], 0, 0, 0);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int i = i0 + wi + 16 * x + g4, j = j0 + wj + 16 * y + li;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = p.alpha * acc[x][y][r];
+                if (p.e) {
+                    float e = 0.f;
+#pragma unroll
+                    for (int s = NP - 1; s >= 0; --s) e += __uint_as_float((unsigned)p.e[s * p.pe + (long long)(i + r) * p.lde + j] << 16);
+                    v += p.beta * e;
+                    if (i + r == j && j < p.rows) v += p.diag;
+                }
+                acc[x][y][r] = v;
+                if (p.out && i + r < p.rows && j < p.cols) store1(p.out, (long long)(i + r) * p.ldo + j, p.dto, v);
+            }
+        }
+    if (p.out) return;
+    // planes leave through LDS, whole rows at a time
+    constexpr int kRow = kTile + 8;
+    ushort_t* sh = reinterpret_cast<ushort_t*>(lds);
+#pragma unroll
+    for (int s = 0; s < NP; ++s) {
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {
+            ushort_t* dst = turn ? p.d2 : p.d1;
+            if (!dst) continue;
+            __syncthreads();
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const int i = wi + 16 * x + g4, j = wj + 16 * y + li;
+                    ushort_t h[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        ushort_t all[NP];
+                        split<NP>(acc[x][y][r], all);
+                        h[r] = all[s];
+                    }
+                    if (turn) {
+                        *reinterpret_cast<uint2*>(sh + j * kRow + i) = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sh[(i + r) * kRow + j] = h[r];
+                    }
+                }
+            __syncthreads();
+            const int ld = turn ? p.ld2 : p.ld1, ro = turn ? j0 : i0, co = turn ? i0 : j0;
+            const long long pl = s * (turn ? p.p2 : p.p1);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int e = threadIdx.x + q * 256, r = e >> 4, c = (e & 15) * 8;
+                *reinterpret_cast<u4*>(dst + pl + (long long)(ro + r) * ld + co + c) = *reinterpret_cast<const u4*>(sh + r * kRow + c);
+            }
+        }
     }
 }
 
@@ -449,7 +599,7 @@ __global__ __launch_bounds__(256) void muon_apply_k(float* __restrict__ p, const
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kAlign = 256;
-int64_t up(int64_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 constexpr int kChip = 256;              // compute units
 
 struct Shape { int64_t m, n; bool tall; };
@@ -458,31 +608,37 @@ Shape shape_of(const dcc_ortho_mat& t) { return Shape{std::min(t.M, t.N), std::m
 // the m x m side in float64: always for small m (its products are latency there), else where n is long enough to pay for their rate
 bool on_square_side(const Shape& s) { return s.m <= 512 || s.n >= 5 * s.m; }
 constexpr int kGroup = 5;               // steps on that side before X X^T is formed anew
+// X <- Q X there in float64 where that takes no longer than splitting X first (at about 50 TFLOP/s, 15 us)
+bool small_apply(const Shape& s) { return 2 * s.m * s.m * s.n < 750000000; }
 
 // tiles of 64 for long depths of X X^T, and then as many depth slices as fill the chip twice, none shorter than 256
 bool wide_gram(const Shape& s) { return s.n >= 4096; }
 int gram_slices(const Shape& s) {
     const int64_t nt = (s.m + 63) / 64, tiles = nt * (nt + 1) / 2;
     if (!wide_gram(s)) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * kChip / tiles, s.n / 256), 128));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(4 * kChip / tiles, s.n / 256), 128));
 }
+int planes_of(int dtype) { return dtype == DCC_ORTHO_BF16 ? 2 : 3; }
+int norm_blocks(const dcc_ortho_mat& t) { return (int)std::max<int64_t>(1, std::min<int64_t>(kNormBlocks, t.M * t.N / 4096)); }
 
 // where a matrix's intermediate results lie in the workspace
-struct Place { int64_t norm, A, B, W, Q0, Q1, Q, X0, X1, part, end; };
-Place place_of(const Shape& s, int steps, int64_t at) {
+struct Place { int64_t norm, A, B, W, Q0, Q1, Qp, Xp, Xt0, Xt1, X0, X1, part, end; };
+Place place_of(const Shape& s, int dtype, int steps, int64_t at) {
     Place p = {};
-    auto take = [&](int64_t bytes) { const int64_t o = at; at += up(bytes); return o; };
-    const int64_t mm = s.m * s.m, mn = 4 * s.m * s.n;
-    p.norm = take(8 * kNormBlocks);
+    auto take = [&](int64_t bytes) { const int64_t o = at; at += up(bytes, kAlign); return o; };
+    const int64_t mq = up(s.m, 16), mp = up(s.m, kTile), np = up(s.n, kTile), mn = 4 * s.m * s.n, np2 = 2 * planes_of(dtype);
     if (on_square_side(s)) {
-        p.A = take(8 * mm); p.B = take(8 * mm); p.W = take(8 * mm); p.Q0 = take(8 * mm); p.Q1 = take(8 * mm); p.Q = take(4 * mm);
-        if (gram_slices(s) > 1) p.part = take(8 * mm * gram_slices(s));
+        p.norm = take(8);
+        p.A = take(8 * mq * mq); p.B = take(8 * mq * mq); p.W = take(8 * mq * mq); p.Q0 = take(8 * mq * mq); p.Q1 = take(8 * mq * mq);
+        if (!small_apply(s)) { p.Qp = take(6 * mp * mp); p.Xt0 = take(6 * mp * np); }
+        if (gram_slices(s) > 1) p.part = take(8 * mq * mq * gram_slices(s));
         if (steps > kGroup) p.X0 = take(mn);
         if (steps > 2 * kGroup) p.X1 = take(mn);
     } else {
-        p.A = take(4 * mm); p.B = take(4 * mm);
-        if (steps > 1) p.X0 = take(mn);
-        if (steps > 2) p.X1 = take(mn);
+        p.norm = take(8 * kNormBlocks);
+        p.A = take(np2 * mp * mp); p.B = take(np2 * mp * mp);
+        p.Xp = take(np2 * mp * np); p.Xt0 = take(np2 * mp * np);
+        if (steps > 1) p.Xt1 = take(np2 * mp * np);
     }
     p.end = at;
     return p;
@@ -494,59 +650,72 @@ const char* list_error(const dcc_ortho_mat* mats, int32_t count, int32_t dtype, 
     if (steps < 1 || steps > DCC_ORTHO_MAX_STEPS) return "steps must lie in 1..32";
     for (int i = 0; i < count; ++i) {
         if (mats[i].M < 0 || mats[i].N < 0) return "negative size";
-        if (mats[i].M > (1 << 30) || mats[i].N > (1 << 30)) return "more than 2^30 rows or columns";
-        if (shape_of(mats[i]).m > 32768) return "both sides over 32768";
+        if (mats[i].M > (1 << 28) || mats[i].N > (1 << 28)) return "more than 2^28 rows or columns";
+        if (shape_of(mats[i]).m > 16384) return "both sides over 16384";
     }
     return nullptr;
 }
 
-// a round: products (of all matrices) that do not depend on each other
-struct Round { std::vector<Prod> x; std::vector<DProd> d, dwide; };
-
-void launch_prods(const std::vector<Prod>& all, float eps, hipStream_t st) {
+// calls f with batches of at most kMaxProds of `all`, their first blocks set from blocks(p)
+template <typename Batch, typename P, typename Blocks, typename F>
+void batches(const std::vector<P>& all, Blocks blocks, F f) {
     for (size_t from = 0; from < all.size(); from += kMaxProds) {
         Batch bt;
         bt.n = (int)std::min<size_t>(kMaxProds, all.size() - from);
-        bt.eps = eps;
-        int64_t big = 0;
-        for (int i = 0; i < bt.n; ++i) {
-            const Prod& p = all[from + i];
-            const int64_t tr = (p.rows + 127) / 128, tc = (p.cols + 127) / 128;
-            big += p.sym ? tr * (tr + 1) / 2 : tr * tc;
-        }
-        // tiles of 128 where they fill the chip, of 64 (more compute units share the depth's latency) where they do not
-        const int tm = big >= kChip ? 128 : 64;
         int64_t first = 0;
         for (int i = 0; i < bt.n; ++i) {
-            Prod& p = bt.p[i] = all[from + i];
-            const int64_t tr = (p.rows + tm - 1) / tm, tc = (p.cols + tm - 1) / tm;
-            p.tcols = (int)tc;
-            p.first = (int)first;
-            first += p.sym ? tr * (tr + 1) / 2 : tr * tc;
+            bt.p[i] = all[from + i];
+            bt.p[i].first = (int)first;
+            first += blocks(bt.p[i]);
         }
-        if (tm == 128) hipLaunchKernelGGL(ortho_prod_k<128>, dim3((unsigned)first), dim3(256), 0, st, bt);
-        else hipLaunchKernelGGL(ortho_prod_k<64>, dim3((unsigned)first), dim3(256), 0, st, bt);
+        f(bt, (unsigned)first);
     }
 }
+int64_t lower(int64_t t) { return t * (t + 1) / 2; }
 
-template <bool WIDE>
-void launch_dprods(const std::vector<DProd>& all, float eps, hipStream_t st) {
+// a round: products (of all matrices) that do not depend on each other
+struct Round {
+    std::vector<Gram> gram[2][2][2];    // [tall][vec][wide]
+    std::vector<Square> square;
+    std::vector<Split> split[2];        // [planes - 2]
+    std::vector<Gemm> gemm[2];
+    std::vector<Apply> apply[2];        // [tall]
+};
+
+template <typename E, bool TALL, bool VEC, bool WIDE>
+void launch_gram(const std::vector<Gram>& all, hipStream_t st) {
     constexpr int tm = WIDE ? 64 : 16;
-    for (size_t from = 0; from < all.size(); from += kMaxProds) {
-        DBatch bt;
-        bt.n = (int)std::min<size_t>(kMaxProds, all.size() - from);
-        bt.eps = eps;
-        int64_t first = 0, longest = 0;
-        for (int i = 0; i < bt.n; ++i) {
-            DProd& p = bt.p[i] = all[from + i];
-            const int64_t t = (p.m + tm - 1) / tm;
-            p.first = (int)first;
-            first += t * (t + 1) / 2 * p.slices;
-            if (p.slices > 1) longest = std::max<int64_t>(longest, (int64_t)p.m * p.m);
-        }
-        hipLaunchKernelGGL(ortho_dprod_k<WIDE>, dim3((unsigned)first), dim3(256), 0, st, bt);
-        if (longest) hipLaunchKernelGGL(ortho_djoin_k, dim3((unsigned)std::min<int64_t>((longest + 255) / 256, 1024), bt.n), dim3(256), 0, st, bt);
-    }
+    batches<GramBatch>(all, [](const Gram& p) { return lower((p.mq + tm - 1) / tm) * p.slices; }, [&](const GramBatch& bt, unsigned blocks) {
+        hipLaunchKernelGGL((ortho_gram_k<E, TALL, VEC, WIDE>), dim3(blocks), dim3(256), 0, st, bt);
+        int64_t longest = 0;
+        for (int i = 0; i < bt.n; ++i)
+            if (bt.p[i].slices > 1) longest = std::max<int64_t>(longest, (int64_t)bt.p[i].mq * bt.p[i].mq);
+        if (longest) hipLaunchKernelGGL(ortho_join_k, dim3((unsigned)std::min<int64_t>((longest + 255) / 256, 1024), bt.n), dim3(256), 0, st, bt);
+    });
+}
+template <typename E>
+void launch_x(const Round& q, hipStream_t st) {         // what reads X: E is its type
+    launch_gram<E, false, false, false>(q.gram[0][0][0], st);
+    launch_gram<E, false, false, true>(q.gram[0][0][1], st);
+    launch_gram<E, false, true, false>(q.gram[0][1][0], st);
+    launch_gram<E, false, true, true>(q.gram[0][1][1], st);
+    launch_gram<E, true, false, false>(q.gram[1][0][0], st);
+    launch_gram<E, true, false, true>(q.gram[1][0][1], st);
+    const auto tiles = [](const Split& p) { return (int64_t)(p.rp / 64) * (p.cp / 64); };
+    batches<SplitBatch>(q.split[0], tiles, [&](const SplitBatch& bt, unsigned n) { hipLaunchKernelGGL((ortho_split_k<E, 2>), dim3(n), dim3(256), 0, st, bt); });
+    batches<SplitBatch>(q.split[1], tiles, [&](const SplitBatch& bt, unsigned n) { hipLaunchKernelGGL((ortho_split_k<E, 3>), dim3(n), dim3(256), 0, st, bt); });
+    const auto quads = [](const Apply& p) { return ((int64_t)((p.rows + 15) / 16) * p.tcols + 3) / 4; };
+    batches<ApplyBatch>(q.apply[0], quads, [&](const ApplyBatch& bt, unsigned n) { hipLaunchKernelGGL((ortho_apply_k<E, false>), dim3(n), dim3(256), 0, st, bt); });
+    batches<ApplyBatch>(q.apply[1], quads, [&](const ApplyBatch& bt, unsigned n) { hipLaunchKernelGGL((ortho_apply_k<E, true>), dim3(n), dim3(256), 0, st, bt); });
+}
+template <int NP>
+bool launch_gemm(const std::vector<Gemm>& all, hipStream_t st) {
+    constexpr int bytes = 2 * 2 * NP * kTile * 4 * 16;
+    if (all.empty()) return true;
+    if (bytes > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(ortho_gemm_k<NP>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    const auto tiles = [](const Gemm& p) { const int64_t t = (p.rows + kTile - 1) / kTile; return p.sym ? lower(t) : t * p.tcols; };
+    batches<GemmBatch>(all, tiles, [&](const GemmBatch& bt, unsigned n) { hipLaunchKernelGGL(ortho_gemm_k<NP>, dim3(n), dim3(256), bytes, st, bt); });
+    return true;
 }
 
 }  // namespace
@@ -557,7 +726,7 @@ DCC_API int64_t dcc_ortho_workspace_bytes(const dcc_ortho_mat* mats, int32_t cou
     if (list_error(mats, count, dtype, steps)) return 0;
     int64_t at = 0;
     for (int i = 0; i < count; ++i)
-        if (mats[i].M > 0 && mats[i].N > 0) at = place_of(shape_of(mats[i]), steps, at).end;
+        if (mats[i].M > 0 && mats[i].N > 0) at = place_of(shape_of(mats[i]), dtype, steps, at).end;
     return at;
 }
 
@@ -566,14 +735,16 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
     if (const char* e = list_error(mats, count, dtype, steps)) return dcc_fail(kEINVAL, std::string("dcc_orthogonalize: ") + e);
     if (!(eps >= 0.f)) return dcc_fail(kEINVAL, "dcc_orthogonalize: eps must not be negative");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+    const int64_t esize = dtype == DCC_ORTHO_F32 ? 4 : 2;
     std::vector<int> live;
     for (int i = 0; i < count; ++i) {
         if (mats[i].M == 0 || mats[i].N == 0) continue;
         if (!mats[i].in || !mats[i].out) return dcc_fail(kEINVAL, "dcc_orthogonalize: null matrix");
+        if ((reinterpret_cast<uintptr_t>(mats[i].in) | reinterpret_cast<uintptr_t>(mats[i].out)) & (esize - 1))
+            return dcc_fail(kEINVAL, "dcc_orthogonalize: a matrix is not aligned to its elements");
         live.push_back(i);
     }
     if (live.empty()) return 0;
-    const int64_t esize = dtype == DCC_ORTHO_F32 ? 4 : 2;
     auto meet = [&](const void* x, const void* y, int64_t nx, int64_t ny) {
         const uintptr_t p = reinterpret_cast<uintptr_t>(x), q = reinterpret_cast<uintptr_t>(y);
         return p < q + ny * esize && q < p + nx * esize;
@@ -586,123 +757,162 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
         }
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))) return dcc_fail(kEINVAL, "dcc_orthogonalize: workspace must be 256-byte aligned");
     char* ws = reinterpret_cast<char*>(workspace);
-    std::vector<Place> place(live.size());
-    std::vector<int> nnorm(live.size());
-    int64_t at = 0;
-    NormBatch nb;
-    nb.n = 0;
-    nb.dtype = dtype;
-    int first = 0;
-    for (size_t i = 0; i < live.size(); ++i) {
-        const dcc_ortho_mat& t = mats[live[i]];
-        place[i] = place_of(shape_of(t), steps, at);
-        at = place[i].end;
-        nnorm[i] = (int)std::min<int64_t>(kNormBlocks, (t.M * t.N + 4095) / 4096);
-        NormMat& m = nb.m[nb.n++];
-        m.x = t.in; m.out = reinterpret_cast<double*>(ws + place[i].norm); m.n = t.M * t.N; m.blocks = nnorm[i]; m.first = first;
-        first += nnorm[i];
-        if (nb.n == kMaxProds * 2 || i + 1 == live.size()) {
-            hipLaunchKernelGGL(ortho_norm_k, dim3(first), dim3(256), 0, st, nb);
-            nb.n = 0;
-            first = 0;
-        }
-    }
-    std::vector<Round> rounds;
+
+    // every matrix's products, round by round; a round's products (of all matrices) run together
+    std::vector<Round> rounds, later;   // later: what reads intermediate X in float32
+    std::vector<NormMat> norms;
     auto round = [&](size_t r) -> Round& {
-        if (rounds.size() <= r) rounds.resize(r + 1);
+        if (rounds.size() <= r) { rounds.resize(r + 1); later.resize(r + 1); }
         return rounds[r];
     };
-    for (size_t i = 0; i < live.size(); ++i) {
-        const dcc_ortho_mat& t = mats[live[i]];
+    int64_t at = 0;
+    for (int idx : live) {
+        const dcc_ortho_mat& t = mats[idx];
         const Shape s = shape_of(t);
-        const Place& pl = place[i];
-        const int m = (int)s.m, n = (int)s.n;
-        const double* norm = reinterpret_cast<const double*>(ws + pl.norm);
-        const void* X = t.in;
-        bool raw = true, flip = false;
+        const Place pl = place_of(s, dtype, steps, at);
+        at = pl.end;
+        const int m = (int)s.m, n = (int)s.n, mq = (int)up(m, 16), mp = (int)up(m, kTile), np = (int)up(n, kTile);
+        const int64_t pmm = (int64_t)mp * mp, pmn = (int64_t)mp * np;
         size_t r = 0;
         int left = steps;
-        auto apply = [&](const float* Q) {      // X <- Q X
-            Prod p = {};
-            const bool last = left == 0;
-            void* out = last ? t.out : static_cast<void*>(ws + (flip ? pl.X1 : pl.X0));
-            flip = !flip;
-            p.alpha = 1.f; p.norm = norm; p.nnorm = nnorm[i];
-            if (s.tall) {       // stored as X^T [n, m]: its rows times the symmetric Q
-                p.a = X; p.dta = raw ? dtype : 0; p.rawa = raw; p.lda = m; p.b = Q; p.ldb = m;
-                p.rows = n; p.cols = m; p.ldo = m;
-            } else {
-                p.a = Q; p.lda = m; p.b = X; p.dtb = raw ? dtype : 0; p.rawb = raw; p.ldb = n; p.bmode = 1;
-                p.rows = m; p.cols = n; p.ldo = n;
-            }
-            p.K = m; p.out = out; p.dto = last ? dtype : 0;
-            round(r++).x.push_back(p);
-            X = out;
-            raw = false;
-        };
         if (on_square_side(s)) {
+            const void* X = t.in;
+            bool raw = true, flip = false;
             double *A = reinterpret_cast<double*>(ws + pl.A), *B = reinterpret_cast<double*>(ws + pl.B), *W = reinterpret_cast<double*>(ws + pl.W);
             double* Qs[2] = {reinterpret_cast<double*>(ws + pl.Q0), reinterpret_cast<double*>(ws + pl.Q1)};
-            float* Qf = reinterpret_cast<float*>(ws + pl.Q);
-            auto square = [&](const double* x, const double* y, void* out) {
-                DProd p = {};
-                p.a = x; p.b = y; p.out = out; p.lda = p.ldb = m; p.m = p.K = m; p.dt = 3; p.slices = 1; p.kper = m; p.alpha = 1.;
+            ushort_t* Qp = small_apply(s) ? nullptr : reinterpret_cast<ushort_t*>(ws + pl.Qp);
+            auto square = [&](const double* x, const double* y, double* out) {
+                Square p = {};
+                p.a = x; p.b = y; p.out = out; p.m = m; p.mq = p.mp = mq; p.alpha = 1.;
                 return p;
             };
+            auto to_planes = [&](Square& p) { p.out = nullptr; p.planes = Qp; p.plane = pmm; p.mp = mp; };
             while (left > 0) {
                 const int groups = (left + kGroup - 1) / kGroup, len = (left + groups - 1) / groups;
                 left -= len;
-                DProd g = {};           // A = X X^T
-                g.a = g.b = X; g.dt = raw ? dtype : 0; g.lda = g.ldb = t.N; g.mode = s.tall; g.m = m; g.K = n; g.out = A; g.alpha = 1.;
-                if (raw) { g.norm = norm; g.nnorm = nnorm[i]; }
+                const bool last = left == 0;
+                double* note = reinterpret_cast<double*>(ws + pl.norm);
+                Scale scale = {};       // after the first p(A), which takes |X|_F^2 from the unscaled A's diagonal and notes it
+                if (raw) scale = Scale{note, 1, 1, eps};
+                Gram g = {};            // A = X X^T
+                g.x = X; g.out = A; g.ld = t.N; g.m = m; g.mq = mq; g.K = n;
                 g.part = reinterpret_cast<double*>(ws + pl.part);
-                g.kper = (n + gram_slices(s) - 1) / gram_slices(s);
-                g.kper = (g.kper + 15) / 16 * 16;
+                g.kper = (int)up((n + gram_slices(s) - 1) / gram_slices(s), 16);
                 g.slices = (n + g.kper - 1) / g.kper;
-                (wide_gram(s) ? round(r).dwide : round(r).d).push_back(g);
+                const int64_t es = raw ? esize : 4;
+                const bool vec = !s.tall && n % 4 == 0 && (reinterpret_cast<uintptr_t>(X) & (4 * es - 1)) == 0;
+                round(r);
+                (raw ? rounds : later)[r].gram[s.tall][vec][wide_gram(s)].push_back(g);
                 ++r;
                 int cur = -1;           // Qs[cur] holds Q
                 for (int k = 0; k < len; ++k) {
                     const bool end = k + 1 == len;
-                    DProd p = square(A, A, k > 0 ? B : end ? static_cast<void*>(Qf) : Qs[0]);       // p(A)
-                    p.alpha = c; p.e = A; p.beta = b; p.diag = a; p.out32 = k == 0 && end;
-                    round(r++).d.push_back(p);
-                    const double* Pk = k > 0 ? B : Qs[0];
-                    if (k > 0) {                            // Q <- p(A) Q
-                        DProd q = square(Pk, Qs[cur], end ? static_cast<void*>(Qf) : Qs[cur ^ 1]);
-                        q.out32 = end;
-                        round(r).d.push_back(q);
+                    Square p = square(A, A, k > 0 ? B : Qs[0]);         // p(A); the first one works on the unscaled A
+                    p.alpha = c; p.e = A; p.beta = b; p.diag = a;
+                    if (k == 0 && raw) { p.s = Scale{A, mq + 1, m, eps}; p.sa = 2; p.note = note; }
+                    if (k == 0 && end && Qp) to_planes(p);
+                    round(r++).square.push_back(p);
+                    double* Pk = k > 0 ? B : Qs[0];
+                    if (k > 0) {                                        // Q <- p(A) Q
+                        Square q = square(Pk, Qs[cur], Qs[cur ^ 1]);
+                        if (end && Qp) to_planes(q);
+                        round(r).square.push_back(q);
                         cur ^= 1;
                         if (end) ++r;
                     } else {
                         cur = 0;
                     }
-                    if (!end) {                             // A <- p(A) A p(A)
-                        round(r++).d.push_back(square(Pk, A, W));
-                        round(r++).d.push_back(square(W, Pk, A));
+                    if (!end) {                                         // A <- p(A) A p(A)
+                        Square w = square(Pk, A, W);
+                        if (k == 0 && raw) { w.s = scale; w.sa = 1; }
+                        round(r++).square.push_back(w);
+                        round(r++).square.push_back(square(W, Pk, A));
                     }
                 }
-                apply(Qf);
+                void* out = last ? t.out : static_cast<void*>(ws + (flip ? pl.X1 : pl.X0));
+                flip = !flip;
+                if (Qp) {
+                    ushort_t* Xt = reinterpret_cast<ushort_t*>(ws + pl.Xt0);        // [np][mp]: X^T
+                    Split sp = {};
+                    sp.x = X; sp.plane = pmn; sp.R = (int)t.M; sp.C = (int)t.N; sp.rp = s.tall ? np : mp; sp.cp = s.tall ? mp : np;
+                    (s.tall ? sp.same : sp.turned) = Xt;
+                    sp.tcols = sp.cp / 64; sp.s = scale;
+                    if (len == 1) ++r;                                  // (not beside the p(A) that notes the norm)
+                    round(r - 1);
+                    (raw ? rounds : later)[r - 1].split[1].push_back(sp);
+                    Gemm q = {};
+                    q.a = s.tall ? Xt : Qp; q.b = s.tall ? Qp : Xt; q.pa = s.tall ? pmn : pmm; q.pb = s.tall ? pmm : pmn;
+                    q.lda = q.ldb = mp; q.K = mp; q.rows = (int)t.M; q.cols = (int)t.N; q.ldo = t.N; q.out = out; q.dto = last ? dtype : 0;
+                    q.tcols = (int)(up(t.N, kTile) / kTile); q.alpha = 1.f;
+                    round(r++).gemm[1].push_back(q);
+                } else {
+                    Apply q = {};
+                    q.x = X; q.q = Qs[cur]; q.out = out; q.ld = t.N; q.m = m; q.mq = mq; q.rows = (int)t.M; q.cols = (int)t.N;
+                    q.tcols = (int)((t.N + 15) / 16); q.dto = last ? dtype : 0; q.s = scale;
+                    round(r);
+                    (raw ? rounds : later)[r++].apply[s.tall].push_back(q);
+                }
+                X = out;
+                raw = false;
             }
         } else {
-            float *A = reinterpret_cast<float*>(ws + pl.A), *B = reinterpret_cast<float*>(ws + pl.B);
+            const int np2 = planes_of(dtype), nb = norm_blocks(t);
+            ushort_t *A = reinterpret_cast<ushort_t*>(ws + pl.A), *B = reinterpret_cast<ushort_t*>(ws + pl.B), *Xp = reinterpret_cast<ushort_t*>(ws + pl.Xp);
+            ushort_t* Xt[2] = {reinterpret_cast<ushort_t*>(ws + pl.Xt0), reinterpret_cast<ushort_t*>(ws + pl.Xt1)};
+            double* norm = reinterpret_cast<double*>(ws + pl.norm);
+            norms.push_back(NormMat{t.in, norm, t.M * t.N, nb, 0});
+            Split sp = {};
+            sp.x = t.in; sp.plane = pmn; sp.R = (int)t.M; sp.C = (int)t.N; sp.rp = s.tall ? np : mp; sp.cp = s.tall ? mp : np;
+            sp.same = s.tall ? Xt[0] : Xp; sp.turned = s.tall ? Xp : Xt[0];
+            sp.tcols = sp.cp / 64; sp.s = Scale{norm, 1, nb, eps};
+            round(r++).split[np2 - 2].push_back(sp);
+            int cur = 0;
             while (left > 0) {
                 --left;
-                Prod g = {};            // A = X X^T
-                g.a = g.b = X; g.dta = g.dtb = raw ? dtype : 0; g.rawa = g.rawb = raw; g.lda = g.ldb = t.N; g.amode = g.bmode = s.tall;
-                g.out = A; g.ldo = m; g.rows = g.cols = m; g.K = n; g.sym = 1; g.alpha = 1.f; g.norm = norm; g.nnorm = nnorm[i];
-                round(r++).x.push_back(g);
-                Prod p = {};            // B = a I + b A + c A^2
-                p.a = p.b = A; p.lda = p.ldb = p.ldo = m; p.out = B; p.rows = p.cols = p.K = m; p.sym = 1; p.alpha = c; p.e = A; p.beta = b; p.diag = a;
-                round(r++).x.push_back(p);
-                apply(B);
+                Gemm g = {};            // A = X X^T
+                g.a = g.b = Xp; g.pa = g.pb = pmn; g.lda = g.ldb = np; g.K = np; g.rows = g.cols = m; g.sym = 1; g.alpha = 1.f;
+                g.d1 = g.d2 = A; g.p1 = g.p2 = pmm; g.ld1 = g.ld2 = mp; g.tcols = mp / kTile;
+                round(r++).gemm[np2 - 2].push_back(g);
+                Gemm p = g;             // B = a I + b A + c A^2
+                p.a = p.b = p.e = A; p.pa = p.pb = p.pe = pmm; p.lda = p.ldb = p.lde = mp; p.K = mp; p.d1 = p.d2 = B; p.alpha = c; p.beta = b; p.diag = a;
+                round(r++).gemm[np2 - 2].push_back(p);
+                Gemm q = {};            // X <- B X
+                q.K = q.lda = q.ldb = mp; q.alpha = 1.f;
+                if (left == 0) {
+                    q.a = s.tall ? Xt[cur] : B; q.b = s.tall ? B : Xt[cur]; q.pa = s.tall ? pmn : pmm; q.pb = s.tall ? pmm : pmn;
+                    q.rows = (int)t.M; q.cols = (int)t.N; q.out = t.out; q.ldo = t.N; q.dto = dtype;
+                } else {                // as [m][n] for the next X X^T, as [n][m] for the next step
+                    q.a = B; q.pa = pmm; q.b = Xt[cur]; q.pb = pmn; q.rows = m; q.cols = n;
+                    q.d1 = Xp; q.p1 = pmn; q.ld1 = np; q.d2 = Xt[cur ^ 1]; q.p2 = pmn; q.ld2 = mp;
+                }
+                q.tcols = (q.cols + kTile - 1) / kTile;
+                round(r++).gemm[np2 - 2].push_back(q);
+                cur ^= 1;
             }
         }
     }
-    for (const Round& q : rounds) {
-        launch_dprods<true>(q.dwide, eps, st);
-        launch_dprods<false>(q.d, eps, st);
-        launch_prods(q.x, eps, st);
+    for (size_t from = 0; from < norms.size(); from += 2 * kMaxProds) {
+        NormBatch nb;
+        nb.n = (int)std::min<size_t>(2 * kMaxProds, norms.size() - from);
+        int first = 0;
+        for (int i = 0; i < nb.n; ++i) {
+            nb.m[i] = norms[from + i];
+            nb.m[i].first = first;
+            first += nb.m[i].blocks;
+        }
+        if (dtype == DCC_ORTHO_F32) hipLaunchKernelGGL(ortho_norm_k<float>, dim3(first), dim3(256), 0, st, nb);
+        else if (dtype == DCC_ORTHO_BF16) hipLaunchKernelGGL(ortho_norm_k<__hip_bfloat16>, dim3(first), dim3(256), 0, st, nb);
+        else hipLaunchKernelGGL(ortho_norm_k<__half>, dim3(first), dim3(256), 0, st, nb);
+    }
+    for (size_t r = 0; r < rounds.size(); ++r) {
+        const Round& q = rounds[r];
+        if (dtype == DCC_ORTHO_F32) launch_x<float>(q, st);
+        else if (dtype == DCC_ORTHO_BF16) launch_x<__hip_bfloat16>(q, st);
+        else launch_x<__half>(q, st);
+        launch_x<float>(later[r], st);
+        batches<SquareBatch>(q.square, [](const Square& p) { return lower(p.mp / 16); },
+                             [&](const SquareBatch& bt, unsigned blocks) { hipLaunchKernelGGL(ortho_square_k, dim3(blocks), dim3(256), 0, st, bt); });
+        if (!launch_gemm<2>(q.gemm[0], st) || !launch_gemm<3>(q.gemm[1], st)) return dcc_fail(kEHIP, "dcc_orthogonalize: shared memory refused");
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string("dcc_orthogonalize: ") + hipGetErrorString(e));
