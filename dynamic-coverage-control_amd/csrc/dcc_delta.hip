@@ -84,6 +84,12 @@ __device__ __forceinline__ void wave_sync() {
 }
 __device__ __forceinline__ f4 mfma(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 zero4() { f4 z = {0.f, 0.f, 0.f, 0.f}; return z; }
+// x, of which the compiler knows nothing: comparisons with it are made where they stand.  (What is compared with the lane's number is the
+// same for all chunks, and would be kept for the whole kernel, as a mask of 64 bits each: more than there are scalar registers.)
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 __device__ __forceinline__ f4 lds4(const float* p) { return *reinterpret_cast<const f4*>(p); }
 
 // sum over the 16 lanes that share lane/16
@@ -108,6 +114,29 @@ __device__ __forceinline__ float state_load(__amdgpu_buffer_rsrc_t rs, unsigned 
 }
 __device__ __forceinline__ void state_store(float v, __amdgpu_buffer_rsrc_t rs, unsigned off) {
     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), rs, off, 0, 0);
+}
+
+// A lane's entries of a state, element (16 t + r, 0) at byte offset off + (16 t + r) * row.  The offsets are counted up here each time: the
+// compiler would otherwise keep all of them in registers for the whole kernel, and spill.
+template <int T, typename F>
+__device__ __forceinline__ void for_state(unsigned off, unsigned row, F f) {
+    off = fresh(off);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            f(t, r, off);
+            off += r < 3 ? row : 13 * row;
+        }
+    }
+}
+template <int T>
+__device__ __forceinline__ void state_load_all(f4 (&s)[T], __amdgpu_buffer_rsrc_t rs, unsigned off, unsigned row) {
+    for_state<T>(off, row, [&](int t, int r, unsigned o) { s[t][r] = state_load(rs, o); });
+}
+template <int T>
+__device__ __forceinline__ void state_store_all(const f4 (&s)[T], __amdgpu_buffer_rsrc_t rs, unsigned off, unsigned row) {
+    for_state<T>(off, row, [&](int t, int r, unsigned o) { state_store(s[t][r], rs, o); });
 }
 
 // ROWS rows of DIMP columns from global memory (row i: base + i * stride; rows >= valid and columns >= dim are zero; valid >= 1) to LDS
@@ -150,25 +179,36 @@ struct RowTile {
 constexpr int kSP = 20;                         // pitch of the 16x16 tiles in LDS (rows 16-byte aligned)
 struct ChunkVec { float beta[kC], gam[kC], toend[kC], seg[kC], gend; float pad[3]; };     // per chunk: gates as the products use them
 
-// The gates of one token as they come from memory
+// The gates of one token as they come from memory (nothing is computed from them here: that would wait for them, and with them for all
+// loads before them) ...
+struct RawGate { float g, beta, m; };
+__device__ __forceinline__ RawGate load_gate(const Seq& p, long long b, int h, long long t) {
+    RawGate x;
+    const float* g = p.g + b * p.sg[1] + h * p.sg[2];
+    const float* be = p.beta + b * p.sb[1] + h * p.sb[2];
+    const float* m = p.masks ? p.masks + b * p.sm[1] : p.g;             // (a select of addresses: no branch)
+    const long long sm = p.masks ? p.sm[0] : 0;
+    t = t < p.T ? t : p.T - 1;
+    x.g = g[t * p.sg[0]];
+    x.beta = be[t * p.sb[0]];
+    x.m = m[t * sm];
+    return x;
+}
+// ... and as they are used: token t >= T does nothing
 struct Gate { float g, beta; int cut; };
-__device__ __forceinline__ Gate load_gate(const Seq& p, long long b, int h, long long t) {
+__device__ __forceinline__ Gate gate_of(const Seq& p, const RawGate& raw, long long t) {
     const bool in = t < p.T;
-    t = in ? t : p.T - 1;
     Gate x;
-    x.g = p.g[t * p.sg[0] + b * p.sg[1] + h * p.sg[2]];
-    x.beta = p.beta[t * p.sb[0] + b * p.sb[1] + h * p.sb[2]];
-    const float m = p.masks ? p.masks[t * p.sm[0] + b * p.sm[1]] : 1.f;
-    x.cut = in && (m == 0.f || x.g < kDead);
-    x.g = x.cut || !in ? 0.f : x.g;
-    x.beta = in ? x.beta : 0.f;
+    x.cut = in && ((p.masks && raw.m == 0.f) || raw.g < kDead);
+    x.g = x.cut || !in ? 0.f : raw.g;
+    x.beta = in ? raw.beta : 0.f;
     return x;
 }
 
 // Decays of one chunk, by one wave: lane l works on token l % 16 (the four groups repeat each other).  Running sums in double: the
 // difference of two float sums would carry the error of the larger one into every D_ij.  Returns this lane's running sum and segment.
 __device__ __forceinline__ void chunk_gates(const Gate& x, int lane, double& run, int& seg, ChunkVec* cv) {
-    const int i = lane & 15;
+    const int i = fresh(lane) & 15;
     double s = (double)x.g;
     int c = x.cut;
 #pragma unroll
@@ -181,7 +221,7 @@ __device__ __forceinline__ void chunk_gates(const Gate& x, int lane, double& run
     seg = c;
     const double send = __shfl(s, 15, 16);
     const int cend = __shfl(c, 15, 16);
-    if (lane < 16) {
+    if (fresh(lane) < 16) {
         const float e = c == 0 ? expf((float)s) : 0.f;
         cv->beta[i] = x.beta;
         cv->gam[i] = e;
@@ -193,6 +233,7 @@ __device__ __forceinline__ void chunk_gates(const Gate& x, int lane, double& run
 
 // D_ij of this lane's four entries (row i = 4*(lane/16) + r, column j = lane % 16), 0 above the diagonal
 __device__ __forceinline__ f4 chunk_decay(double run, int seg, int lane) {
+    lane = fresh(lane);
     const int j = lane & 15, g4 = (lane >> 4) << 2;
     f4 d;
 #pragma unroll
@@ -208,6 +249,7 @@ __device__ __forceinline__ f4 chunk_decay(double run, int seg, int lane) {
 // (I + L)^-1 -> `t` [16][kSP]; this lane holds L[4*(lane/16) + r][lane % 16], strictly lower triangular.  Lane l solves column l % 16 by
 // forward substitution; the entries of L come by lane reads, so nothing waits on memory.
 __device__ __forceinline__ void unit_lower_inverse(const f4& L, float* t, int lane) {
+    lane = fresh(lane);
     const int c = lane & 15;
     float x[kC];
 #pragma unroll
@@ -266,7 +308,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
     ChunkVec* cvs = reinterpret_cast<ChunkVec*>(Ti + BT * kC * kSP);
     float* Qs = reinterpret_cast<float*>(cvs + BT);
     float* Am = Qs + BT * kC * KP;              // [BT][16][kSP] (Q K^T) . D
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g4 = (lane >> 4) << 2;
     const long long bh = blockIdx.x, b = bh / p.H;
     const int h = (int)(bh - b * p.H), hk = h / p.rep;
@@ -315,7 +357,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
             for (int r = 0; r < 4; ++r) state_store(S[t][r], rs, soff + (16 * t + r) * srow);
     };
     RowTile<E, BT * kC, DKP, 64 * NW, VEC> rk, rq;
-    Gate gate[CPW];
+    RawGate gate[CPW];
     E vnext[4];
     auto valid_of = [&](int c0) {
         const long long left = p.T - (long long)c0 * kC;
@@ -351,7 +393,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
         if (HASQ) rq.commit(Qs, KP, valid, p.DK, 1.f);
         Gate now[CPW];
 #pragma unroll
-        for (int n = 0; n < CPW; ++n) now[n] = gate[n];
+        for (int n = 0; n < CPW; ++n) now[n] = gate_of(p, gate[n], t0 + (wave + n * NW) * kC + li);
         __syncthreads();
         if (i + 1 < nblk) fetch(block(i + 1));
 #pragma unroll
@@ -493,58 +535,75 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
 
 // States at the segment starts from the segments' summaries: S <- P S + N, one 16-column tile per workgroup, wave w the rows 16 w..;
 // the state passes through LDS (one barrier a segment) while the next P and N are loading.  `back`: from the last segment to the first.
-template <int DKT>
+template <int DKT, bool VEC>
 __global__ __launch_bounds__(64 * DKT) void delta_join_k(const Seq p, int back) {
     __shared__ float sh[2][DKT * 16][17];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g4 = (lane >> 4) << 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g4 = (lane >> 4) << 2;
     const long long bh = blockIdx.x, sst = (long long)p.DK * p.DV, spp = (long long)p.DK * p.DK;
     const int col = blockIdx.y * 16 + li, n = p.nseg - 1;
     const unsigned srow = 4u * p.DV, off = col < p.DV ? 4u * ((16 * wave + g4) * p.DV + col) : kOutside;
     const int prow = 16 * wave + li;
-    f4 P[DKT], N;
     // summary i belongs to segment i (forward) or i + 1 (backward)
-    auto fetch = [&](int i, bool withP) {
+    struct Sum { f4 P[DKT], N; };
+    auto fetch = [&](Sum& s, int i) {
+        i = back ? n - 1 - i : i;
+        i = i < 0 ? 0 : i < n ? i : n - 1;
         const __amdgpu_buffer_rsrc_t rn = state_rsrc(p.sumN + (bh * n + i) * sst, p.DK, p.DV), rp = state_rsrc(p.sumP + (bh * n + i) * spp, p.DK, p.DK);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) N[r] = state_load(rn, off + r * srow);
-        if (!withP) return;
+        for (int r = 0; r < 4; ++r) s.N[r] = state_load(rn, off + r * srow);
 #pragma unroll
-        for (int t = 0; t < DKT; ++t)
+        for (int t = 0; t < DKT; ++t) {
+            const int k = 16 * t + g4;
+            if constexpr (VEC) {        // DK a multiple of four
+                s.P[t] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rp, k < p.DK ? 4u * (prow * p.DK + k) : kOutside, 0, 0));
+            } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int k = 16 * t + g4 + r;
-                P[t][r] = state_load(rp, k < p.DK ? 4u * (prow * p.DK + k) : kOutside);
+                for (int r = 0; r < 4; ++r) s.P[t][r] = state_load(rp, k + r < p.DK ? 4u * (prow * p.DK + k + r) : kOutside);
             }
+        }
     };
-    fetch(back ? n - 1 : 0, false);
-    f4 S = N;
-    for (int i = 0; i < n; ++i) {
+    f4 S;
+    auto leave = [&](int i) {           // the state after i + 1 summaries, to LDS and to its segment
         float (*x)[17] = sh[i & 1];
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[16 * wave + g4 + r][li] = S[r];
-        const int seg = back ? n - 1 - i : i + 1;       // the segment that this state enters
-        const __amdgpu_buffer_rsrc_t ro = state_rsrc(p.segS + (bh * p.nseg + seg) * sst, p.DK, p.DV);
+        const __amdgpu_buffer_rsrc_t ro = state_rsrc(p.segS + (bh * p.nseg + (back ? n - 1 - i : i + 1)) * sst, p.DK, p.DV);
 #pragma unroll
         for (int r = 0; r < 4; ++r) state_store(S[r], ro, off + r * srow);
-        if (i + 1 == n) break;
-        fetch(back ? n - 2 - i : i + 1, true);
         __syncthreads();
+    };
+    auto step = [&](const Sum& s, int i) {
+        const float (*x)[17] = sh[i & 1];
         // a segment with a restart has P == 0, and then what the state held before (NaN included) is gone: not multiplied
-        bool any = false;
+        unsigned any = 0;               // (bits: 0 and -0 are zero, NaN is not)
 #pragma unroll
         for (int t = 0; t < DKT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) any |= P[t][r] != 0.f;
-        if (!__any(any)) { S = N; continue; }
-        f4 a = N, c = zero4();
+            for (int r = 0; r < 4; ++r) any |= __float_as_uint(s.P[t][r]);
+        if (!__any((any & 0x7fffffffu) != 0)) { S = s.N; return; }
+        f4 a = s.N, c = zero4();
 #pragma unroll
         for (int t = 0; t < DKT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; r += 2) {
-                a = mfma(P[t][r], x[16 * t + g4 + r][li], a);
-                c = mfma(P[t][r + 1], x[16 * t + g4 + r + 1][li], c);
+                a = mfma(s.P[t][r], x[16 * t + g4 + r][li], a);
+                c = mfma(s.P[t][r + 1], x[16 * t + g4 + r + 1][li], c);
             }
         S = a + c;
+    };
+    Sum s0, s1;                         // one on its way while the other is used
+    fetch(s1, 0);
+    fetch(s0, 1);
+    S = s1.N;
+    for (int i = 0; i < n; i += 2) {
+        leave(i);
+        if (i + 1 == n) break;
+        fetch(s1, i + 2);
+        step(s0, i);
+        leave(i + 1);
+        if (i + 2 == n) break;
+        fetch(s0, i + 3);
+        step(s1, i + 1);
     }
 }
 
@@ -577,7 +636,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     float* redb = Zm + kC * kSP;                // [2][3][NW][16]: dbeta, v.dv, q.dq by wave
     float* dotb = redb + 2 * 3 * NW * 16;       // [2][NW]: <dS, S> at the chunk's end
     ChunkTiles* tiles = reinterpret_cast<ChunkTiles*>(dotb + 2 * NW);       // [2]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g4 = (lane >> 4) << 2;
     const long long bh = blockIdx.x, b = bh / p.H;
     const int h = (int)(bh - b * p.H), hk = h / p.rep;
@@ -600,7 +659,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     E vnext[TPW][4];
     RowTile<E, kC, DKP, 64 * NW, VEC> rk, rq;
     RowTile<E, kC, DVP, 64 * NW, VEC> ro;
-    Gate gate;
+    RawGate gate;
     auto valid_of = [&](int c) {
         const long long left = p.T - (long long)c * kC;
         return left < kC ? (int)left : kC;
@@ -609,10 +668,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p.DK, p.DV);
 #pragma unroll
         for (int w = 0; w < TPW; ++w)
-#pragma unroll
-            for (int t = 0; t < DKT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) S0[w][t][r] = state_load(rs, soff[w] + (16 * t + r) * srow);
+            state_load_all(S0[w], rs, soff[w], srow);
     };
     auto fetch_v = [&](int c) {
 #pragma unroll
@@ -697,10 +753,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const __amdgpu_buffer_rsrc_t rs = state_rsrc(from, p.DK, p.DV);
 #pragma unroll
         for (int w = 0; w < TPW; ++w)
-#pragma unroll
-            for (int t = 0; t < DKT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) dS[w][t][r] = state_load(rs, soff[w] + (16 * t + r) * srow);
+            state_load_all(dS[w], rs, soff[w], srow);
     }
     const int last = cend - 1;
     if (last >= cbeg) {
@@ -708,7 +761,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         fetch_state(cend);
         dot_state(last & 1);
         commit_rows(last);
-        const Gate gt = gate;
+        const Gate gt = gate_of(p, gate, (long long)last * kC + li);
         __syncthreads();
         fetch_state(last);
         fetch_v(last);
@@ -725,7 +778,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const float* Os = Ob + par * kC * VP;
         const ChunkTiles& ct = tiles[par];
         float* red = redb + par * 3 * NW * 16;
-        const Gate gnext = gate;
+        const Gate gnext = gate_of(p, gate, t0 - kC + li);
         if (c > cbeg) commit_rows(c - 1);
         if (c > cbeg + 1) fetch_rows(c - 2);
         const f4 be = lds4(ct.cv.beta + g4), ga = lds4(ct.cv.gam + g4), de = lds4(ct.cv.toend + g4);
@@ -905,24 +958,29 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             qd[r] = row_sum(qd[r]);
             if (li == 0) red[(2 * NW + wave) * 16 + g4 + r] = qd[r];
         }
+        float dot = 0.f;                // (before the barrier: the next chunk's dot_state writes there)
+        if (wave == 0) {
+#pragma unroll
+            for (int i = 0; i < NW; ++i) dot += dotb[par * NW + i];
+        }
         __syncthreads();
-        if (wave == 0) {        // (the others go on: red, dotb and the tiles alternate)
-            float sb = 0.f, w = 0.f, dot = 0.f;
+        if (wave == 0) {        // (the others go on: red and the tiles alternate)
+            float sb = 0.f, w = 0.f;
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 sb += red[i * 16 + li];
                 w += red[(2 * NW + i) * 16 + li] - red[(NW + i) * 16 + li];
-                dot += dotb[par * NW + i];
             }
             const float sraw = ct.cv.seg[li];
             const bool cut = sraw < 0.f;
             const float seg = cut ? -1.f - sraw : sraw;
             const float send = __shfl(seg, 15, 16);
             float acc = seg == send ? dot : 0.f;
+            const int lc = fresh(li);
 #pragma unroll
             for (int s = kC - 1; s >= 0; --s) {
                 const float ws = __shfl(w, s, 16), ss = __shfl(seg, s, 16);
-                if (s >= li && ss == seg) acc += ws;
+                if (s >= lc && ss == seg) acc += ws;
             }
             const long long t = t0 + li;
             if (lane < kC && t < p.T) {
@@ -935,12 +993,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const __amdgpu_buffer_rsrc_t rs = state_rsrc(p.dstate0 + bh * sst, p.DK, p.DV);
 #pragma unroll
         for (int w = 0; w < TPW; ++w)
-            if (wave + w * NW < DVT) {
-#pragma unroll
-                for (int t = 0; t < DKT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) state_store(dS[w][t][r], rs, soff[w] + (16 * t + r) * srow);
-            }
+            if (wave + w * NW < DVT) state_store_all(dS[w], rs, soff[w], srow);
     }
 }
 
@@ -1122,7 +1175,9 @@ template <typename E, int DKT, int DIR>
 int segments(const Seq& p, hipStream_t st) {
     const int rc = p.vec ? launch_walk<E, DKT, 4, 4, true, DIR>(p, st) : launch_walk<E, DKT, 1, 4, false, DIR>(p, st);
     if (rc != 0) return rc;
-    hipLaunchKernelGGL((delta_join_k<DKT>), dim3((unsigned)(p.B * p.H), (p.DV + 15) / 16), dim3(64 * DKT), 0, st, p, DIR == SUM_BWD);
+    const dim3 grid((unsigned)(p.B * p.H), (p.DV + 15) / 16);
+    if (p.DK % 4 == 0) hipLaunchKernelGGL((delta_join_k<DKT, true>), grid, dim3(64 * DKT), 0, st, p, DIR == SUM_BWD);
+    else hipLaunchKernelGGL((delta_join_k<DKT, false>), grid, dim3(64 * DKT), 0, st, p, DIR == SUM_BWD);
     return done("gated delta rule");
 }
 template <typename E, int DKT>
