@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "dcc_internal.h"
@@ -980,6 +981,25 @@ unsigned number(Batch<P>& bt, int n, Blocks blocks) {
     bt.first[kMaxProds] = (int)first;
     return (unsigned)first;
 }
+// does an output share bytes with an input or with another output?  (a list may hold thousands of matrices: sorted, not pair by pair)
+bool outputs_meet(const dcc_ortho_mat* mats, const std::vector<int>& live, int64_t esize) {
+    typedef std::pair<uintptr_t, uintptr_t> Range;
+    auto range = [&](const void* p, int i) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+        return Range(a, a + mats[i].M * mats[i].N * esize);
+    };
+    std::vector<Range> outs;
+    for (int i : live) outs.push_back(range(mats[i].out, i));
+    std::sort(outs.begin(), outs.end());
+    for (size_t i = 1; i < outs.size(); ++i)
+        if (outs[i].first < outs[i - 1].second) return true;
+    for (int i : live) {
+        const Range r = range(mats[i].in, i);
+        const auto next = std::lower_bound(outs.begin(), outs.end(), Range(r.second, 0));        // the first output from r's end on
+        if (next != outs.begin() && (next - 1)->second > r.first) return true;
+    }
+    return false;
+}
 // calls f with batches of at most kMaxProds of `all` and their numbers of blocks and descriptions
 template <typename P, typename Blocks, typename F>
 void batches(const std::vector<P>& all, Blocks blocks, F f) {
@@ -1086,16 +1106,7 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
         live.push_back(i);
     }
     if (live.empty()) return 0;
-    auto meet = [&](const void* x, const void* y, int64_t nx, int64_t ny) {
-        const uintptr_t p = reinterpret_cast<uintptr_t>(x), q = reinterpret_cast<uintptr_t>(y);
-        return p < q + ny * esize && q < p + nx * esize;
-    };
-    for (int i : live)
-        for (int j : live) {
-            const int64_t ni = mats[i].M * mats[i].N, nj = mats[j].M * mats[j].N;
-            if (meet(mats[i].out, mats[j].in, ni, nj) || (i != j && meet(mats[i].out, mats[j].out, ni, nj)))
-                return dcc_fail(kEINVAL, "dcc_orthogonalize: an output overlaps an input or another output");
-        }
+    if (outputs_meet(mats, live, esize)) return dcc_fail(kEINVAL, "dcc_orthogonalize: an output overlaps an input or another output");
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))) return dcc_fail(kEINVAL, "dcc_orthogonalize: workspace must be 256-byte aligned");
     char* ws = reinterpret_cast<char*>(workspace);
 

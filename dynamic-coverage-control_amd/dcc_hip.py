@@ -875,7 +875,8 @@ def gated_delta_bwd(q, k, v, g, beta, masks, scale, ckpt, dout, dstate=None):
 
 def gated_delta_step(q, k, v, g, beta, state, masks=None, scale=None, out=None, state_out=None):
     """One token of the gated delta rule (rollout, serving): q, k [B,HK,DK], v [B,H,DV], g, beta [B,H], state [B,H,DK,DV] float32,
-    masks [B] or None.  out [B,H,DV] and state_out (contiguous; `state` itself: updated in place) are allocated when absent.
+    masks [B] or None.  out [B,H,DV] and state_out (contiguous; `state` itself: updated in place) are allocated when absent, and lie
+    apart from the operands and from each other.
     -> o, new state.  No gradient (the training pass is fused.gated_delta).  No CPU path."""
     if state is None:
         raise ValueError("gated_delta_step: a state is needed")

@@ -10,6 +10,7 @@
  *   dcc_delta_fwd     T tokens: o and the last state; optionally the states the gradient starts from (`ckpt`)
  *   dcc_delta_bwd     its gradient for q, k, v, g, beta and the first state
  *   dcc_delta_step    one token (rollout, serving): the state is read and written once, in place if state1 == state0
+ *                     (o and state1 lie apart from the operands and from each other)
  *
  * Layout: time-major.  q, k: [T, B, HK, DK], v, o: [T, B, H, DV] in `dtype` (float32, bfloat16 or float16), H a multiple of HK: value
  * head h reads key head h / (H / HK).  g (log decay, <= 0 in use), beta: [T, B, H] float32; masks: [T, B] float32 or NULL (no restarts).

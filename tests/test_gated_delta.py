@@ -7,6 +7,7 @@ the state update, each 2^-24 of the largest magnitude in play, and the updates o
     2^-24 * (4 T + 2 DK + 64) * max|ref|          (gradients, a second recurrence over the first one's results: 4 times that),
 16-bit results to half a step of their type on top (bf16 2^-8, fp16 2^-11 of the value)."""
 import ctypes
+import math
 import itertools
 
 import pytest
@@ -474,3 +475,15 @@ def test_binding_refuses():
         dcc_hip.gated_delta_step(*one, big[:n].view_as(d["state"]), state_out=big[n // 2:n // 2 + n].view_as(d["state"]))
     with pytest.raises(ValueError):
         dcc_hip.gated_delta_step(*one, d["state"], state_out=torch.empty(3, device="cuda"))
+    # results over operands
+    flat = torch.zeros(4096, device="cuda")
+    oshape, sshape = one[2].shape, d["state"].shape
+    at = lambda start, shape: flat[start:start + math.prod(shape)].view(shape)
+    v = at(0, oshape)
+    for bad in (dict(out=v), dict(out=at(8, oshape)), dict(state_out=at(v.numel() - 1, sshape)),
+                dict(out=at(1024, oshape), state_out=at(1024 + 4, sshape))):
+        with pytest.raises(dcc_hip.DccError, match="apart"):
+            dcc_hip.gated_delta_step(one[0], one[1], v, one[3], one[4], d["state"], **bad)
+    with pytest.raises(dcc_hip.DccError, match="apart"):
+        dcc_hip.gated_delta_step(*one, at(0, sshape), out=at(16, oshape))
+    dcc_hip.gated_delta_step(one[0], one[1], v, one[3], one[4], d["state"], out=at(v.numel(), oshape), state_out=d["state"])

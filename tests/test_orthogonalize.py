@@ -64,6 +64,11 @@ def test_entry_points_validate_before_touching_the_device():
         assert b"dcc_orthogonalize" in L.dcc_last_error()
     two = (dcc_hip.OrthoMat * 2)(dcc_hip.OrthoMat(a, a + 4096, 4, 4), dcc_hip.OrthoMat(a + 64, a + 4096, 4, 4))
     assert go(two, 2) == -1                                     # two results in one place
+    far = [dcc_hip.OrthoMat(a + 64 * i, a + 4096 + 64 * i, 4, 4) for i in range(5)]
+    far[3].out = a + 64 * 4 + 60                                # the last bytes of the last input
+    assert go((dcc_hip.OrthoMat * 5)(*far), 5) == -1 and b"overlaps" in L.dcc_last_error()
+    far[3].out, far[0].inp = a + 4096 + 64 * 9, a + 4096 + 64 * 9 - 4      # an input that ends inside an output
+    assert go((dcc_hip.OrthoMat * 5)(*far), 5) == -1 and b"overlaps" in L.dcc_last_error()
     assert L.dcc_ortho_workspace_bytes(one(), 1, 0, 0) == 0
 
 
@@ -99,6 +104,32 @@ def test_steps(steps, shape):
     G = gradient_like(*shape, seed=steps).cuda()
     check(dcc_hip.orthogonalize(G, steps=steps), reference(G, steps))
     check(dcc_hip.orthogonalize(G, steps=steps, coeffs=(1.875, -1.25, 0.375)), reference(G, steps, (1.875, -1.25, 0.375)))
+
+
+# large and nearly square (step by step), and long (many tiles of X <- Q X): rows of a multiple of four or not, either way round
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(705, 705), (720, 901), (1030, 772), (200, 16388), (200, 16389), (16388, 200), (16389, 201)], ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_large(shape, dtype):
+    import dcc_hip
+    G = gradient_like(*shape, dtype=dtype, seed=shape[1]).cuda()
+    check(dcc_hip.orthogonalize(G), reference(G), "%dx%d" % shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(720, 901), (200, 16388), (16389, 201)], ids=lambda s: "%dx%d" % s)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_in_two_groups_and_off_alignment(shape, dtype):
+    """six steps (X X^T is formed twice on the m x m side), from and to places that are aligned to one element only"""
+    import dcc_hip
+    G = gradient_like(*shape, dtype=dtype, seed=7)
+    n = G.numel()
+    src, dst = torch.zeros(n + 1, dtype=dtype, device="cuda"), torch.zeros(n + 2, dtype=dtype, device="cuda")
+    src[1:].copy_(G.reshape(-1))
+    X, out = src[1:].view(shape), dst[1:-1].view(shape)
+    dcc_hip.orthogonalize(X, steps=6, out=out)
+    check(out, reference(G, 6), "%dx%d" % shape)
+    assert float(dst[0]) == 0.0 and float(dst[-1]) == 0.0
 
 
 @pytest.mark.gpu
