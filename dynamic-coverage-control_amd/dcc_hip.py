@@ -4,6 +4,7 @@ host code and the hand-written HIP kernels.
 There is NO CPU fallback: if the shared library is missing or no HIP device is visible, loading /
 creating raises.  Tensors are torch CUDA(=HIP) tensors; only their data_ptr() crosses the ABI.
 """
+import contextlib
 import ctypes
 import os
 
@@ -159,8 +160,11 @@ def _ptr(t):
     return None if t is None else _vp(t.data_ptr())
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # without building a Stream object for every launch
+
+
 def _stream():
-    return _vp(torch.cuda.current_stream().cuda_stream)
+    return _vp(_raw_stream(torch.cuda.current_device()) if _raw_stream else torch.cuda.current_stream().cuda_stream)
 
 
 def bytes_per_step(n_agents, n_pois, with_actions=True, with_obs=True):
@@ -784,44 +788,45 @@ _DELTA_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _delta_seq(what, q, k, v, g, beta, state, masks, scale, lead):
-    """Checks the operands (lead: number of leading axes, 2 = [T, B, ..], 1 = [B, ..]) and fills dcc_delta_seq.
-    -> (struct, operands to keep alive)"""
+    """Checks the operands (lead: number of leading axes, 2 = [T, B, ..], 1 = [B, ..]) and fills dcc_delta_seq."""
     if not (torch.is_tensor(v) and v.is_cuda):
         raise DccError("%s: v is not on a HIP device (there is no CPU path)" % what)
     if v.dtype not in _DELTA_DTYPES:
         raise ValueError("%s: v must be float32, bfloat16 or float16, not %s" % (what, v.dtype))
     if v.dim() != lead + 2 or not torch.is_tensor(q) or q.dim() != lead + 2:
         raise ValueError("%s: q and v must have %d axes" % (what, lead + 2))
-    rows, (HK, DK), (H, DV) = tuple(v.shape[:lead]), tuple(q.shape[lead:]), tuple(v.shape[lead:])
+    rows, (HK, DK), (H, DV) = v.shape[:lead], q.shape[lead:], v.shape[lead:]
     if not (HK >= 1 and H >= 1 and H % HK == 0 and 1 <= DK <= DELTA_MAX_DIM and 1 <= DV <= DELTA_MAX_DIM):
         raise ValueError("%s: %d value heads of %d over %d key heads of %d (a multiple; sizes 1..%d)" % (what, H, DV, HK, DK, DELTA_MAX_DIM))
-    want = [("q", q, rows + (HK, DK), v.dtype), ("k", k, rows + (HK, DK), v.dtype), ("v", v, rows + (H, DV), v.dtype),
-            ("g", g, rows + (H,), torch.float32), ("beta", beta, rows + (H,), torch.float32)]
-    if masks is not None:
-        want.append(("masks", masks, rows, torch.float32))
-    if state is not None:
-        want.append(("state", state, (rows[-1], H, DK, DV), torch.float32))
-    for name, t, shape, dt in want:
-        if not torch.is_tensor(t) or tuple(t.shape) != shape or t.dtype != dt or t.device != v.device:
-            raise ValueError("%s: %s must be %s %s on %s" % (what, name, shape, dt, v.device))
+    dt, f32, device, keys, gates = v.dtype, torch.float32, v.get_device(), rows + (HK, DK), rows + (H,)
+
+    def check(name, t, shape, dtype, last=False):
+        if not torch.is_tensor(t) or t.shape != shape or t.dtype != dtype or t.get_device() != device:
+            raise ValueError("%s: %s must be %s %s on %s" % (what, name, tuple(shape), dtype, v.device))
+        st = t.stride()
         # (an axis of one element says nothing by its stride)
-        if name in ("q", "k", "v") and t.shape[-1] > 1 and t.stride(-1) != 1:
+        if last and shape[-1] > 1 and st[-1] != 1:
             raise ValueError("%s: the last axis of %s must be contiguous" % (what, name))
-    if state is not None and not state.is_contiguous():
-        raise ValueError("%s: state must be contiguous" % what)
-    s = DeltaSeq()
-    s.T, s.B, s.HK, s.H, s.DK, s.DV = (rows[0] if lead == 2 else 1), rows[-1], HK, H, DK, DV
-    s.dtype, s.scale = _DELTA_DTYPES[v.dtype], float(DK ** -0.5 if scale is None else scale)
-    s.q, s.k, s.v, s.g, s.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
-    s.masks = None if masks is None else masks.data_ptr()
-    s.state0 = None if state is None else state.data_ptr()
+        return pad + (st[:-1] if last else st)
+
     pad = (0,) if lead == 1 else ()
-    for name, t in (("st_q", q), ("st_k", k), ("st_v", v)):
-        setattr(s, name, (ctypes.c_int64 * 3)(*(pad + tuple(t.stride()[:-1]))))
-    s.st_g, s.st_beta = (ctypes.c_int64 * 3)(*(pad + tuple(g.stride()))), (ctypes.c_int64 * 3)(*(pad + tuple(beta.stride())))
-    if masks is not None:
-        s.st_masks = (ctypes.c_int64 * 2)(*(pad + tuple(masks.stride())))
-    return s
+    st = [check("q", q, keys, dt, True), check("k", k, keys, dt, True), check("v", v, v.shape, dt, True), check("g", g, gates, f32),
+          check("beta", beta, gates, f32), (0, 0) if masks is None else check("masks", masks, rows, f32)]
+    if state is not None:
+        check("state", state, (rows[-1], H, DK, DV), f32)
+        if not state.is_contiguous():
+            raise ValueError("%s: state must be contiguous" % what)
+    return DeltaSeq(rows[0] if lead == 2 else 1, rows[-1], HK, H, DK, DV, _DELTA_DTYPES[dt], float(DK ** -0.5 if scale is None else scale),
+                    q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), None if masks is None else masks.data_ptr(),
+                    None if state is None else state.data_ptr(), *st)
+
+
+def _on(t):
+    """The device of t as the current one (nothing to do when it is: a rollout asks for every step)."""
+    return _HERE_ALREADY if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_HERE_ALREADY = contextlib.nullcontext()
 
 
 def _delta_ws(n, device):
@@ -835,7 +840,7 @@ def gated_delta_fwd(q, k, v, g, beta, state=None, masks=None, scale=None, want_c
     -> o [T,B,H,DV], last state [B,H,DK,DV], what gated_delta_bwd starts from (None unless want_ckpt).  No CPU path."""
     s = _delta_seq("gated_delta_fwd", q, k, v, g, beta, state, masks, scale, 2)
     L = load_library()
-    with torch.cuda.device(v.device):
+    with _on(v):
         o = torch.empty(v.shape, dtype=v.dtype, device=v.device)
         last = torch.empty((s.B, s.H, s.DK, s.DV), dtype=torch.float32, device=v.device)
         ckpt = _delta_ws(max(1, L.dcc_delta_ckpt_floats(ctypes.byref(s))), v.device) if want_ckpt else None
@@ -860,7 +865,7 @@ def gated_delta_bwd(q, k, v, g, beta, masks, scale, ckpt, dout, dstate=None):
     need = max(1, L.dcc_delta_ckpt_floats(ctypes.byref(s)))
     if not torch.is_tensor(ckpt) or ckpt.dtype != torch.float32 or ckpt.numel() != need or ckpt.device != v.device or not ckpt.is_contiguous():
         raise ValueError("gated_delta_bwd: ckpt must be the %d floats that gated_delta_fwd(want_ckpt=True) returned for these sizes" % need)
-    with torch.cuda.device(v.device):
+    with _on(v):
         mk = lambda shape, dt: torch.empty(shape, dtype=dt, device=v.device)
         dq, dk, dv = mk(q.shape, q.dtype), mk(k.shape, k.dtype), mk(v.shape, v.dtype)
         dg, dbeta, ds = mk(g.shape, torch.float32), mk(beta.shape, torch.float32), mk(shape, torch.float32)
@@ -886,7 +891,7 @@ def gated_delta_step(q, k, v, g, beta, state, masks=None, scale=None, out=None, 
             raise ValueError("gated_delta_step: %s must be contiguous %s %s on %s" % (name, tuple(shape), dt, v.device))
     if state_out is not None and state_out.data_ptr() != state.data_ptr() and _overlap(state, state_out):
         raise ValueError("gated_delta_step: state_out must be state itself or lie apart from it")
-    with torch.cuda.device(v.device):
+    with _on(v):
         out = torch.empty(v.shape, dtype=v.dtype, device=v.device) if out is None else out
         state_out = torch.empty_like(state) if state_out is None else state_out
         s.o, s.state1 = out.data_ptr(), state_out.data_ptr()
@@ -928,7 +933,7 @@ def orthogonalize(mats, steps=5, coeffs=NEWTON_SCHULZ, eps=1e-7, out=None):
         raise ValueError("orthogonalize: coeffs = (a, b, c)")
     L = load_library()
     dt = _DELTA_DTYPES[ref.dtype]
-    with torch.cuda.device(ref.device):
+    with _on(ref):
         if outs is None:
             outs = [torch.empty_like(t) for t in ms]
         flat = []
@@ -951,7 +956,7 @@ def muon_momentum(grad, buf, direction, momentum, nesterov=True, clip=None):
         _f32c(t, nm)
         if t.numel() != grad.numel() or t.device != grad.device:
             raise ValueError("muon_momentum: %s has %d elements on %s, grad %d on %s" % (nm, t.numel(), t.device, grad.numel(), grad.device))
-    with torch.cuda.device(grad.device):
+    with _on(grad):
         _check(load_library().dcc_muon_momentum(_ptr(grad), _ptr(buf), _ptr(direction), grad.numel(), float(momentum), int(bool(nesterov)),
                                                 _ptr(clip), _stream()), "dcc_muon_momentum")
 
@@ -967,5 +972,5 @@ def muon_apply(param, direction, segs, keep=1.0):
         if s[0] < end or s[0] + s[1] > param.numel():
             raise ValueError("muon_apply: ranges must lie apart from each other and within %d elements" % param.numel())
         end = s[0] + s[1]
-    with torch.cuda.device(param.device):
+    with _on(param):
         _check(load_library().dcc_muon_apply(_ptr(param), _ptr(direction), arr, len(segs), float(keep), _stream()), "dcc_muon_apply")
