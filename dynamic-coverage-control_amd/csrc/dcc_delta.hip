@@ -1027,7 +1027,7 @@ __global__ __launch_bounds__(256) void delta_fold_k(const float* __restrict__ a,
 
 // ---- one token -----------------------------------------------------------------------------------------------------------------
 // Bound by reading and writing the state once: 32768 x 4 states of 64 x 64 in 835 us, 5.3 TB/s, where a large copy reaches 4.7; 1000 x 6 states
-// of 96 x 80 in 70 us.  64 x 4 states take 23 us, all of it the caller's launch.  A wave owns one (row, head) and 16 * VEC value columns; lane l holds columns
+// of 96 x 80 in 70 us.  64 x 4 states take 4.5 us.  A wave owns one (row, head) and 16 * VEC value columns; lane l holds columns
 // VEC * (l % 16).. of the key rows 4 i + l / 16, all of them loaded before the first use.
 template <typename E, int R, int VEC>
 __global__ __launch_bounds__(256) void delta_step_k(const Seq p, int slices) {

@@ -78,9 +78,10 @@ __device__ __forceinline__ int which(const Batch<P>& bt, int blk) {
     return pi;
 }
 
-// Consecutive workgroups go to the eight dies in turn: numbered so, each die gets a run of neighbours, which share operands in its L2.  The
-// grid is a multiple of eight; numbers from first[kMaxProds] on have no work.
-__device__ __forceinline__ int die_order() { return (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3); }
+// Consecutive workgroups go to the eight dies in turn: numbered so, each die gets a run of neighbouring tiles of every product, which share
+// operands in its L2.  A product has a multiple of eight workgroups; those numbered from `tiles` on have no work.  (Runs over a whole launch
+// would give the long products to some dies: 2048 x 2048, 1000 x 2500 and 4096 x 1024 together, X <- B X in 134 us, 112 so.)
+__device__ __forceinline__ int die_order(int blk, int tiles) { return (blk & 7) * ((tiles + 7) >> 3) + (blk >> 3); }
 
 // tile (ti, tj), tj <= ti, of the lower triangle counted row by row
 __device__ __forceinline__ void lower_tile(int blk, int& ti, int& tj) {
@@ -142,7 +143,7 @@ struct Gram {                           // out = X X^T, X [m, K] in memory as [m
     const void* x;
     double *out, *part;                 // part: [slices][mq * mq] where slices > 1
     long long ld;
-    int m, mq, K, slices, kper;         // kper: a multiple of 32
+    int m, mq, K, slices, kper, tiles;  // kper: a multiple of 32
 };
 using GramBatch = Batch<Gram>;
 
@@ -259,13 +260,12 @@ __global__ __launch_bounds__(64 * kWaves) void ortho_gram_k(const GramBatch bt) 
 // MFMA, which is busy in two cycles of three: 256 x 165952 float32 in 259 us, 47 TFLOP/s of the 77 that the instruction alone reaches.
 template <typename E, bool TALL, bool VEC>
 __global__ __launch_bounds__(256, 2) void ortho_gram_wide_k(const GramBatch bt) {
-    const int id = die_order();         // a die's workgroups share slices of X, in its L2
-    if (id >= bt.first[kMaxProds]) return;
-    const int pi = which(bt, id);
+    const int pi = which(bt, blockIdx.x);
     const Gram& p = bt.p[pi];
     const E* x = reinterpret_cast<const E*>(p.x);
-    const int blk = id - bt.first[pi], m = p.m, mq = p.mq, nt = (mq + 63) / 64, tiles = nt * (nt + 1) / 2, slice = blk / tiles;
+    const int blk = die_order(blockIdx.x - bt.first[pi], p.tiles), m = p.m, mq = p.mq, nt = (mq + 63) / 64, tiles = nt * (nt + 1) / 2, slice = blk / tiles;
     const long long ld = p.ld;
+    if (blk >= p.tiles) return;
     int ti, tj;
     lower_tile(blk - slice * tiles, ti, tj);
     // (turned by the slice, so that what is above the diagonal is not always the same SIMD's)
@@ -444,7 +444,7 @@ struct Apply {                          // out [rows][cols] = Q X (wide: X [m][n
     const double* q;
     void* out;
     long long ld;                       // of X and out
-    int m, mq, rows, cols, tcols, dto;
+    int m, mq, rows, cols, tcols, dto, tiles;
     Scale s;
 };
 using ApplyBatch = Batch<Apply>;
@@ -494,12 +494,11 @@ __global__ __launch_bounds__(64 * kWaves) void ortho_apply_k(const ApplyBatch bt
 template <typename E, bool TALL, bool VEC>
 __global__ __launch_bounds__(256, 2) void ortho_apply_wide_k(const ApplyBatch bt) {
     __shared__ double red[8];
-    const int id = die_order();         // (along the shorter side first, like the plane products: neighbours share X or Q)
-    if (id >= bt.first[kMaxProds]) return;
-    const int pi = which(bt, id);
+    const int pi = which(bt, blockIdx.x);
     const Apply& p = bt.p[pi];
     const E* x = reinterpret_cast<const E*>(p.x);
-    const int m = p.m, mq = p.mq, rows = p.rows, cols = p.cols, blk = id - bt.first[pi], trows = (rows + 63) / 64;
+    const int m = p.m, mq = p.mq, rows = p.rows, cols = p.cols, blk = die_order(blockIdx.x - bt.first[pi], p.tiles), trows = (rows + 63) / 64;
+    if (blk >= p.tiles) return;         // (tiles along the shorter side first, like the plane products: neighbours share X or Q)
     const int ti = TALL ? blk / p.tcols : blk % trows, tj = TALL ? blk - ti * p.tcols : blk / trows;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, g = lane >> 4;
     const int i0 = ti * 64 + (wave >> 1) * 32, j0 = tj * 128 + (wave & 1) * 64, jl = j0 + 4 * li;
@@ -663,7 +662,7 @@ struct Gemm {                           // v = alpha A B^T + beta E + diag I
     void* out;                          // or, bounded by rows and cols, v itself
     long long ldo;                      // row length of out
     int lda, ldb, lde, ld1, ld2, K,     // depths of the planes' rows; of this product
-         rows, cols, dto, sym, tcols;
+         rows, cols, dto, sym, tcols, tiles;
     float alpha, beta, diag;
 };
 using GemmBatch = Batch<Gemm>;
@@ -701,11 +700,10 @@ __global__ __launch_bounds__(512) void ortho_gemm_k(const GemmBatch bt) {
     constexpr int kSlice = kTile * 4 * NP;              // 16-byte pieces of one operand's slice
     constexpr int kStage = 2 * kSlice, NS = kAhead<NP> + 1;
     extern __shared__ u4 lds[];                         // [NS][2][kSlice]
-    const int id = die_order();
-    if (id >= bt.first[kMaxProds]) return;
-    const int pi = which(bt, id);
+    const int pi = which(bt, blockIdx.x);
     const Gemm& p = bt.p[pi];
-    const int blk = id - bt.first[pi];
+    const int blk = die_order(blockIdx.x - bt.first[pi], p.tiles);
+    if (blk >= p.tiles) return;
     int ti, tj;
     if (p.sym) {
         lower_tile(blk, ti, tj);
@@ -1011,7 +1009,7 @@ void batches(const std::vector<P>& all, Blocks blocks, F f) {
         f(bt, sum, n);
     }
 }
-unsigned in_eights(unsigned n) { return (n + 7) / 8 * 8; }
+int64_t in_eights(int64_t n) { return (n + 7) / 8 * 8; }
 int64_t lower(int64_t t) { return t * (t + 1) / 2; }
 int64_t square_tiles(const Square& p, int d) { return lower((p.mq + d - 1) / d); }
 constexpr unsigned kFewTiles = 80;      // fewer tiles of 32 x 32 than that in a launch: tiles of 16 x 16 (one 256 x 256, 36 or 72 of them: 103 us in all
@@ -1034,8 +1032,8 @@ void launch_gram(const std::vector<Gram>& all, hipStream_t st) {
 }
 template <typename E, bool TALL, bool VEC>
 void launch_gram_wide(const std::vector<Gram>& all, hipStream_t st) {
-    batches(all, [](const Gram& p) { return lower((p.mq + 63) / 64) * p.slices; }, [&](const GramBatch& bt, unsigned blocks, int n) {
-        hipLaunchKernelGGL((ortho_gram_wide_k<E, TALL, VEC>), dim3(in_eights(blocks)), dim3(256), 0, st, bt);
+    batches(all, [](const Gram& p) { return in_eights(p.tiles); }, [&](const GramBatch& bt, unsigned blocks, int n) {
+        hipLaunchKernelGGL((ortho_gram_wide_k<E, TALL, VEC>), dim3(blocks), dim3(256), 0, st, bt);
         int64_t longest = 0;
         for (int i = 0; i < n; ++i)
             if (bt.p[i].slices > 1) longest = std::max<int64_t>(longest, (int64_t)bt.p[i].mq * bt.p[i].mq);
@@ -1044,8 +1042,8 @@ void launch_gram_wide(const std::vector<Gram>& all, hipStream_t st) {
 }
 template <typename E, bool TALL, bool VEC>
 void launch_apply_wide(const std::vector<Apply>& all, hipStream_t st) {
-    batches(all, [](const Apply& p) { return (int64_t)((p.rows + 63) / 64) * p.tcols; }, [&](const ApplyBatch& bt, unsigned blocks, int) {
-        hipLaunchKernelGGL((ortho_apply_wide_k<E, TALL, VEC>), dim3(in_eights(blocks)), dim3(256), 0, st, bt);
+    batches(all, [](const Apply& p) { return in_eights(p.tiles); }, [&](const ApplyBatch& bt, unsigned blocks, int) {
+        hipLaunchKernelGGL((ortho_apply_wide_k<E, TALL, VEC>), dim3(blocks), dim3(256), 0, st, bt);
     });
 }
 template <typename E>
@@ -1072,9 +1070,14 @@ bool launch_gemm(const std::vector<Gemm>& all, hipStream_t st) {
     constexpr int bytes = (kAhead<NP> + 1) * 2 * NP * kTile * 4 * 16;
     if (all.empty()) return true;
     if (bytes > 65536 && hipFuncSetAttribute(reinterpret_cast<const void*>(ortho_gemm_k<NP>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
-    const auto tiles = [](const Gemm& p) { const int64_t t = (p.rows + kTile - 1) / kTile; return p.sym ? lower(t) : t * p.tcols; };
-    batches(all, tiles, [&](const GemmBatch& bt, unsigned n, int) {
-        hipLaunchKernelGGL(ortho_gemm_k<NP>, dim3(in_eights(n)), dim3(512), bytes, st, bt);
+    std::vector<Gemm> longest = all;     // first: what starts last is short
+    std::stable_sort(longest.begin(), longest.end(), [](const Gemm& x, const Gemm& y) { return x.K > y.K; });
+    for (Gemm& p : longest) {
+        const int64_t t = (p.rows + kTile - 1) / kTile;
+        p.tiles = (int)(p.sym ? lower(t) : t * p.tcols);
+    }
+    batches(longest, [](const Gemm& p) { return in_eights(p.tiles); }, [&](const GemmBatch& bt, unsigned n, int) {
+        hipLaunchKernelGGL(ortho_gemm_k<NP>, dim3(n), dim3(512), bytes, st, bt);
     });
     return true;
 }
@@ -1148,6 +1151,7 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
                 g.part = reinterpret_cast<double*>(ws + pl.part);
                 g.kper = (int)up((n + gram_slices(s) - 1) / gram_slices(s), 32);
                 g.slices = (n + g.kper - 1) / g.kper;
+                g.tiles = (int)(lower((mq + 63) / 64) * g.slices);
                 const int64_t es = raw ? esize : 4;
                 const bool vec = !s.tall && n % 4 == 0 && (reinterpret_cast<uintptr_t>(X) & (4 * es - 1)) == 0;
                 round(r);
@@ -1184,6 +1188,7 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
                 const int64_t ds = last ? esize : 4;
                 const bool vec4 = t.N % 4 == 0 && (reinterpret_cast<uintptr_t>(X) & (4 * es - 1)) == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * ds - 1)) == 0;
                 q.tcols = (int)((t.N + (wide ? 127 : 31)) / (wide ? 128 : 32));
+                q.tiles = (int)((t.M + 63) / 64) * q.tcols;             // (of the wide form)
                 round(r);
                 Round& to = (raw ? rounds : later)[r++];
                 (wide ? to.wide_apply[s.tall][vec4] : to.apply[s.tall]).push_back(q);
