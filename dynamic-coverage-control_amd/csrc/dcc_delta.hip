@@ -431,7 +431,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
 #pragma unroll
                 for (int r = 0; r < 4; ++r) vv[r] = full && tc + g4 + r < p.T ? Elem<E>::get(vnext[r]) : 0.f;
                 if (MODE == SUM_BWD ? c0 + c > cbeg : c0 + c + 1 < cend) fetch_v(MODE == SUM_BWD ? tc - kC : tc + kC);
-                if (MODE == FULL && p.ckpt) store_state(p.ckpt + (bh * (p.nchunk + 1) + c0 + c) * sst);
+                if (MODE == FULL && p.ckpt) store_state(p.ckpt + (bh * p.nchunk + c0 + c) * sst);
                 const float* kr = Ks + (c * kC + li) * KP + g4;
                 const float* qr = Qs + (c * kC + li) * KP + g4;
                 const ChunkVec& cv = cvs[c];
@@ -535,7 +535,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
         store_state(unit ? p.sumP + at * p.DK * p.DK : p.sumN + at * sst);
     } else if (seg == p.nseg - 1) {
         if (p.state_out) store_state(p.state_out + bh * sst);
-        if (p.ckpt) store_state(p.ckpt + (bh * (p.nchunk + 1) + p.nchunk) * sst);
     }
 }
 
@@ -620,9 +619,10 @@ __global__ __launch_bounds__(64 * DKT) void delta_join_k(const Seq p, int back) 
 //   dS <- gam_C dS + Q^T (gam do) - K^T (gam X)                                                                    (by value columns)
 //   dQ = gam do S0^T + (do U^T . D) K                                                                              (by key columns)
 //   dK = (do U^T . D)^T Q + D_C U dS^T - gam X S0^T + (Z + Z^T) K,   Z = -(X U^T . D), strictly lower              (by key columns)
-//   dg_t = sum over s >= t of the same segment (q_s.dq_s - v_s.dv_s), + <dS_C, S_C> if no restart follows in the chunk
-// (the last line sums <dS', S'> from the chunk's end, where it is taken whole: no running sum crosses a chunk).  S0 comes from the
-// checkpoints of the forward pass; U, X, dS pass through LDS where the contraction changes from key to value columns.  Between the two
+//   dg_t = <dS'_t, S'_t> = gam_C <dS_C, S0> + sum over s >= t of gam_s (q_s.(S0 do_s) - k_s.(S0 x_s)) + sum over j < t of D_Cj k_j.(dS_C u_j)
+//          + sum over s >= t > j of D_sj ((q_s.k_j)(do_s.u_j) - (k_s.k_j)(x_s.u_j))
+// (every term holds the decay of token t: dg_t of a head that forgets fast is as small as exp(g_t), and a difference of larger sums, such as
+// q.dq - v.dv, would have no digits of it left.)  S0 comes from the checkpoints of the forward pass; U, X, dS pass through LDS where the contraction changes from key to value columns.  Between the two
 // halves, waves 0 and 1 form do U^T and X U^T while waves 2 and 3 prepare the state-free part of the chunk that comes next; its rows were
 // loaded one chunk ahead.  Three barriers per chunk.
 // Bound by the chains between those barriers: two workgroups a compute unit (LDS: 67 KB at 64 x 64), 28 thousand cycles a chunk, of which the
@@ -643,8 +643,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     float* dSs = Xs + kC * VP;                  // [DKP][VP]
     float* Bm = dSs + DKP * VP;                 // (do U^T) . D
     float* Zm = Bm + kC * kSP;                  // Z + Z^T
-    float* redb = Zm + kC * kSP;                // [2][3][NW][16]: dbeta, v.dv, q.dq by wave
-    float* dotb = redb + 2 * 3 * NW * 16;       // [2][NW]: <dS, S> at the chunk's end
+    float* redb = Zm + kC * kSP;                // [2][4][NW][16] by wave: dbeta; dg's pairs (waves 0 and 1), terms of s, terms of j
+    float* dotb = redb + 2 * 4 * NW * 16;       // [2][NW]: <dS_C, S0>
     ChunkTiles* tiles = reinterpret_cast<ChunkTiles*>(dotb + 2 * NW);       // [2]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g4 = (lane >> 4) << 2;
@@ -656,7 +656,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     const E* dou = reinterpret_cast<const E*>(p.dout) + b * p.sdo[1] + h * p.sdo[2];
     const long long sst = (long long)p.DK * p.DV, st = p.B * p.H;
     const unsigned srow = 4u * p.DV;
-    const float* ck0 = p.ckpt + bh * (p.nchunk + 1) * sst;
+    const float* ck0 = p.ckpt + bh * p.nchunk * sst;
     const int seg = blockIdx.y, cbeg = seg * p.seglen, cend = cbeg + p.seglen < p.nchunk ? cbeg + p.seglen : p.nchunk;
     unsigned soff[TPW];
 #pragma unroll
@@ -742,7 +742,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             for (int r = 0; r < 4; ++r) ct.Am[(g4 + r) * kSP + li] = g4 + r >= li ? D[r] * m0[r] : 0.f;
         }
     };
-    auto dot_state = [&](int par) {             // this wave's part of <dS, S0> -> dotb[par]
+    auto dot_state = [&](int par) {             // this wave's part of <dS_C, S0> -> dotb[par]
         float d = 0.f;
 #pragma unroll
         for (int w = 0; w < TPW; ++w)
@@ -768,8 +768,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     const int last = cend - 1;
     if (last >= cbeg) {
         fetch_rows(last);
-        fetch_state(cend);
-        dot_state(last & 1);
         commit_rows(last);
         const Gate gt = gate_of(p, gate, (long long)last * kC + li);
         __syncthreads();
@@ -787,13 +785,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const float* Qs = Qb + par * kC * KP;
         const float* Os = Ob + par * kC * VP;
         const ChunkTiles& ct = tiles[par];
-        float* red = redb + par * 3 * NW * 16;
+        float* red = redb + par * 4 * NW * 16;
         const Gate gnext = gate_of(p, gate, t0 - kC + li);
         if (c > cbeg) commit_rows(c - 1);
         if (c > cbeg + 1) fetch_rows(c - 2);
         const f4 be = lds4(ct.cv.beta + g4), ga = lds4(ct.cv.gam + g4), de = lds4(ct.cv.toend + g4);
         const float ge = ct.cv.gend;
-        float db[4] = {0.f, 0.f, 0.f, 0.f}, vd[4] = {0.f, 0.f, 0.f, 0.f};
+        float db[4] = {0.f, 0.f, 0.f, 0.f};
+        dot_state(par);
 #pragma unroll
         for (int w = 0; w < TPW; ++w) {
             const int tile = wave + w * NW, col = tile * 16 + li;
@@ -841,7 +840,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             for (int r = 0; r < 4; ++r) {
                 x[r] = be[r] * y[r];
                 db[r] += y[r] * (rhat[r] - nu[r]);
-                vd[r] += vv[r] * x[r];
                 Us[(g4 + r) * VP + tile * 16 + li] = u[r];
                 Xs[(g4 + r) * VP + tile * 16 + li] = x[r];
                 if (mine && t0 + g4 + r < p.T) dv[r * st * p.DV] = Elem<E>::put(x[r]);
@@ -863,13 +861,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
                 for (int t = 0; t < DKT; ++t) dS[w][t] = mfma(kc[r * KP + 16 * t], x[r], dS[w][t]);
         }
-        dot_state(par ^ 1);                     // for the chunk before this one
         if (c > cbeg) { fetch_state(c - 1); fetch_v(c - 1); }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             db[r] = row_sum(db[r]);
-            vd[r] = row_sum(vd[r]);
-            if (li == 0) { red[wave * 16 + g4 + r] = db[r]; red[(NW + wave) * 16 + g4 + r] = vd[r]; }
+            if (li == 0) red[wave * 16 + g4 + r] = db[r];
         }
         __syncthreads();
         if (wave < 2) {         // wave 0: do U^T, wave 1: X U^T
@@ -883,10 +879,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
                 for (int r = 0; r < 4; r += 2) { m0 = mfma(a[r], e[r], m0); m1 = mfma(a[r + 1], e[r + 1], m1); }
             }
             m0 = m0 + m1;
+            const int lc = fresh(li);
+            f4 pair, sum = zero4();     // the pairs (s, j) of dg; their sums over s >= t
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = g4 + r;
                 const float D = ct.Dm[i * kSP + li];
+                const float w = wave == 0 ? ct.Am[i * kSP + li] : -ct.Nm[i * kSP + li];
+                pair[r] = i > lc ? w * m0[r] : 0.f;
                 if (wave == 0) {
                     Bm[i * kSP + li] = i >= li ? D * m0[r] : 0.f;
                 } else if (i >= li) {
@@ -895,12 +895,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
                     Zm[li * kSP + i] = z;
                 }
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum = mfma(g4 + r >= lc ? 1.f : 0.f, pair[r], sum);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float w = row_sum(lc < g4 + r ? sum[r] : 0.f);
+                if (li == 0) red[(NW + wave) * 16 + g4 + r] = w;
+            }
         } else if (wave < 4 && c > cbeg) {
             prepare(c - 1, wave - 2, gnext);
         }
         __syncthreads();
         const __amdgpu_buffer_rsrc_t rs = state_rsrc(ck0 + c * sst, p.DK, p.DV);
-        float qd[4] = {0.f, 0.f, 0.f, 0.f};
+        float ps[4] = {0.f, 0.f, 0.f, 0.f}, pj[4] = {0.f, 0.f, 0.f, 0.f};     // dg's terms of s and of j
 #pragma unroll
         for (int w = 0; w < KPW; ++w) {
             const int tile = wave + w * NW, kcol = tile * 16 + li;
@@ -935,14 +942,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             }
             const f4 bm = lds4(Bm + li * kSP + g4), zm = lds4(Zm + li * kSP + g4);
             f4 dq, dk;
+            float kvs[4], qvs[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
+                const float kv = kvs[r] = Ks[(g4 + r) * KP + kcol], qv = qvs[r] = Qs[(g4 + r) * KP + kcol];
+                const float u = de[r] * gu[r], x = ga[r] == 0.f ? 0.f : ga[r] * gx[r];
                 dq[r] = ga[r] == 0.f ? 0.f : ga[r] * gq[r];
-                dk[r] = de[r] * gu[r] - (ga[r] == 0.f ? 0.f : ga[r] * gx[r]);
+                dk[r] = u - x;
+                ps[r] += dq[r] * qv - x * kv;
+                pj[r] += u * kv;
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float kv = Ks[(g4 + r) * KP + kcol], qv = Qs[(g4 + r) * KP + kcol];
+                const float kv = kvs[r], qv = qvs[r];
                 dq = mfma(bm[r], kv, dq);
                 dk = mfma(Bm[(g4 + r) * kSP + li], qv, dk);
                 dk = mfma(zm[r], kv, dk);
@@ -950,7 +962,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             const long long at = ((t0 + g4) * st + bh) * p.DK + kcol;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                qd[r] += dq[r] * Qs[(g4 + r) * KP + kcol];
                 if (mine && t0 + g4 + r < p.T) {
                     const long long i = at + r * st * p.DK;
                     if (p.dq32) {       // heads that share a key head: summed afterwards, in a fixed order
@@ -965,32 +976,27 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            qd[r] = row_sum(qd[r]);
-            if (li == 0) red[(2 * NW + wave) * 16 + g4 + r] = qd[r];
-        }
-        float dot = 0.f;                // (before the barrier: the next chunk's dot_state writes there)
-        if (wave == 0) {
-#pragma unroll
-            for (int i = 0; i < NW; ++i) dot += dotb[par * NW + i];
+            ps[r] = row_sum(ps[r]);
+            pj[r] = row_sum(pj[r]);
+            if (li == 0) { red[(2 * NW + wave) * 16 + g4 + r] = ps[r]; red[(3 * NW + wave) * 16 + g4 + r] = pj[r]; }
         }
         __syncthreads();
-        if (wave == 0) {        // (the others go on: red and the tiles alternate)
-            float sb = 0.f, w = 0.f;
+        if (wave == 0) {        // (the others go on: red, dotb and the tiles alternate)
+            float sb = 0.f, ws = 0.f, wj = 0.f, dot = 0.f;
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 sb += red[i * 16 + li];
-                w += red[(2 * NW + i) * 16 + li] - red[(NW + i) * 16 + li];
+                ws += red[(2 * NW + i) * 16 + li];
+                wj += red[(3 * NW + i) * 16 + li];
+                dot += dotb[par * NW + i];
             }
-            const float sraw = ct.cv.seg[li];
-            const bool cut = sraw < 0.f;
-            const float seg = cut ? -1.f - sraw : sraw;
-            const float send = __shfl(seg, 15, 16);
-            float acc = seg == send ? dot : 0.f;
+            const bool cut = ct.cv.seg[li] < 0.f;
+            float acc = red[NW * 16 + li] + red[(NW + 1) * 16 + li] + (ge == 0.f ? 0.f : ge * dot);
             const int lc = fresh(li);
 #pragma unroll
             for (int s = kC - 1; s >= 0; --s) {
-                const float ws = __shfl(w, s, 16), ss = __shfl(seg, s, 16);
-                if (s >= lc && ss == seg) acc += ws;
+                const float a = __shfl(ws, s, 16), b = __shfl(wj, s, 16);
+                acc += s >= lc ? a : b;
             }
             const long long t = t0 + li;
             if (lane < kC && t < p.T) {
@@ -1208,7 +1214,7 @@ int fwd_typed(const Seq& p, hipStream_t st) {
 template <typename E, int DKT, int DVT, int NW, bool VEC>
 int launch_bwd(const Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, VP = DVT * 16 + 4;
-    const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 6 * NW * 16 + 2 * NW) + 2 * sizeof(ChunkTiles);
+    const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 8 * NW * 16 + 2 * NW) + 2 * sizeof(ChunkTiles);
     if (!allow_lds(delta_bwd_k<E, DKT, DVT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_bwd: shared memory refused");
     hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3((unsigned)(p.B * p.H), p.nseg), dim3(64 * NW), lds, st, p);
     return done("dcc_delta_bwd");
@@ -1273,7 +1279,7 @@ extern "C" {
 
 DCC_API int64_t dcc_delta_ckpt_floats(const dcc_delta_seq* s) {
     if (sizes_error(s)) return 0;
-    return s->B * s->H * ((s->T + kC - 1) / kC + 1) * (int64_t)s->DK * s->DV;
+    return s->B * s->H * ((s->T + kC - 1) / kC) * (int64_t)s->DK * s->DV;
 }
 DCC_API int64_t dcc_delta_fwd_workspace_floats(const dcc_delta_seq* s) {
     int len;

@@ -70,7 +70,7 @@ typedef struct {
     float *dstate0;              /* contiguous, or NULL */
 } dcc_delta_grad;
 
-/* Floats of `ckpt` for these sizes (the state at the start of every chunk of 16 tokens, and the last); 0 for sizes that are refused. */
+/* Floats of `ckpt` for these sizes (the state at the start of every chunk of 16 tokens); 0 for sizes that are refused. */
 DCC_API int64_t dcc_delta_ckpt_floats(const dcc_delta_seq* s);
 /* Floats of `workspace` of dcc_delta_fwd / dcc_delta_bwd (0: none needed; NULL is then allowed). */
 DCC_API int64_t dcc_delta_fwd_workspace_floats(const dcc_delta_seq* s);
