@@ -177,7 +177,7 @@ struct RowTile {
 };
 
 constexpr int kSP = 20;                         // pitch of the 16x16 tiles in LDS (rows 16-byte aligned)
-struct ChunkVec { float beta[kC], gam[kC], toend[kC], seg[kC], gend; float pad[3]; };     // per chunk: gates as the products use them
+struct ChunkVec { float beta[kC], gam[kC], toend[kC], seg[kC], g[kC], gend; int odd; float pad[2]; };     // per chunk: gates as the products use them
 
 // The gates of one token as they come from memory (nothing is computed from them here: that would wait for them, and with them for all
 // loads before them) ...
@@ -227,6 +227,7 @@ __device__ __forceinline__ void chunk_gates(const Gate& x, int lane, double& run
         cv->gam[i] = e;
         cv->toend[i] = c == cend ? expf((float)(send - s)) : 0.f;
         cv->seg[i] = x.cut ? -1.f - c : (float)c;         // sign: a restart at this token
+        cv->g[i] = x.g;
         if (i == 15) cv->gend = e;
     }
 }
@@ -286,6 +287,45 @@ __device__ __forceinline__ void chunk_products(const float* kr, const float* qr,
     }
     kk = k0 + k1;
     qk = q0 + q1;
+}
+
+// ---- values that are not finite ------------------------------------------------------------------------------------------------
+// The products of a chunk meet every token with every other: what is not finite would reach tokens before it and tokens behind a restart,
+// by way of 0 * NaN.  A chunk whose results are not all finite is therefore taken again, token by token: these are its pieces, for a lane's
+// part of a state, rows 16 t + 4 * (lane / 16) + r of one column.  (Anything in the inputs that is not finite shows in the results: every
+// update of a chunk is a sum over all its tokens.)  The barriers to the scheduler keep the registers of these rare paths few.
+__device__ __forceinline__ float not_finite(const f4& x) { return (x[0] * 0.f + x[1] * 0.f) + (x[2] * 0.f + x[3] * 0.f); }      // 0, or NaN
+template <int T>
+__device__ __forceinline__ float token_dot(const f4 (&S)[T], const float* row) {         // S^T row; row: LDS, at + 4 * (lane / 16)
+    float a = 0.f;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const f4 x = lds4(row + 16 * t);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a += x[r] * S[t][r];
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    a += __shfl_xor(a, 16, 64);
+    return a + __shfl_xor(a, 32, 64);
+}
+template <int T>
+__device__ __forceinline__ void token_add(f4 (&S)[T], const float* row, float u) {        // S += row u^T
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const f4 x = lds4(row + 16 * t);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][r] += x[r] * u;
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+template <int T>
+__device__ __forceinline__ void token_decay(f4 (&S)[T], const ChunkVec& cv, int i) {
+    const bool cut = cv.seg[i] < 0.f;
+    const float al = expf(cv.g[i]);
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][r] = cut ? 0.f : al * S[t][r];
 }
 
 // ---- forward -------------------------------------------------------------------------------------------------------------------
@@ -413,12 +453,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
             chunk_products<DKT, HASQ>(Ks + (c * kC + li) * KP + g4, Qs + (c * kC + li) * KP + g4, kk, qk);
             wave_sync();
             const f4 be = lds4(cvs[c].beta + g4);
+            float amod = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int j = g4 + r;
                 L[r] = j > li ? be[r] * D[r] * kk[r] : 0.f;
-                if (HASQ) Am[(c * kC + j) * kSP + li] = j >= li ? D[r] * qk[r] : 0.f;
+                if (HASQ) {
+                    const float a = j >= li ? D[r] * qk[r] : 0.f;
+                    Am[(c * kC + j) * kSP + li] = a;
+                    if (MODE == SUM_BWD) amod += a * 0.f;
+                }
             }
+            // (forward, a query reaches its own token's row only)
+            const bool odd = __any(not_finite(L) + amod != 0.f);
+            if (lane == 0) cvs[c].odd = odd;
             unit_lower_inverse(L, Ti + c * kC * kSP, lane);
         }
         __syncthreads();
@@ -437,6 +485,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
                 const ChunkVec& cv = cvs[c];
                 const f4 be = lds4(cv.beta + g4), ga = lds4(cv.gam + g4), de = lds4(cv.toend + g4);
                 const float ge = cv.gend;
+                const int odd = cv.odd;
                 const float* kc = Ks + (c * kC + g4) * KP + li;
                 const float* qc = Qs + (c * kC + g4) * KP + li;
                 f4 ks = zero4(), qs = zero4();
@@ -453,6 +502,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
                     f4 y = zero4();
 #pragma unroll
                     for (int r = 0; r < 4; ++r) ks[r] = (ks[r] + qs[r]) * de[r];
+                    if (__builtin_expect(odd | __any(not_finite(ks) + not_finite(vv) != 0.f), 0)) {
+#pragma unroll 1
+                        for (int at = (valid - c * kC < kC ? valid - c * kC : kC) - 1; at >= 0; --at) {
+                            const float* kt = Ks + (c * kC + at) * KP + g4;
+                            const int r = at & 3;
+                            const float x = __shfl(r == 0 ? vv[0] : r == 1 ? vv[1] : r == 2 ? vv[2] : vv[3], 4 * (at - r) + li, 64);
+                            if (!unit) token_add(S, Qs + (c * kC + at) * KP + g4, x);
+                            token_add(S, kt, -cv.beta[at] * token_dot(S, kt));
+                            token_decay(S, cv, at);
+                        }
+                        continue;
+                    }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) ks = mfma(Am[(c * kC + g4 + r) * kSP + li], vv[r], ks);
 #pragma unroll
@@ -495,26 +556,42 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
                     rhs[r] = be[r] * (vv[r] - (ga[r] == 0.f ? 0.f : ga[r] * ks[r]));
                     out[r] = ga[r] == 0.f ? 0.f : ga[r] * qs[r];
                 }
-                const f4 ti = lds4(Ti + (c * kC + li) * kSP + g4);
-                f4 u = zero4();
+                if (__builtin_expect(odd | __any(not_finite(rhs) != 0.f), 0)) {
+#pragma unroll 1
+                    for (int at = 0; at < valid - c * kC && at < kC; ++at) {
+                        const float* kt = Ks + (c * kC + at) * KP + g4;
+                        const int r = at & 3;
+                        const float x = __shfl(r == 0 ? vv[0] : r == 1 ? vv[1] : r == 2 ? vv[2] : vv[3], 4 * (at - r) + li, 64);
+                        token_decay(S, cv, at);
+                        token_add(S, kt, cv.beta[at] * (x - token_dot(S, kt)));
+                        if (MODE == FULL) {
+                            const float y = token_dot(S, Qs + (c * kC + at) * KP + g4);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) u = mfma(ti[r], rhs[r], u);
-                f4 ud;
+                            for (int e = 0; e < 4; ++e) out[e] = g4 + e == at ? y : out[e];
+                        }
+                    }
+                } else {
+                    const f4 ti = lds4(Ti + (c * kC + li) * kSP + g4);
+                    f4 u = zero4();
 #pragma unroll
-                for (int r = 0; r < 4; ++r) ud[r] = u[r] * de[r];
-                if (MODE == FULL) {
-                    const f4 am = lds4(Am + (c * kC + li) * kSP + g4);
+                    for (int r = 0; r < 4; ++r) u = mfma(ti[r], rhs[r], u);
+                    f4 ud;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) out = mfma(am[r], u[r], out);
+                    for (int r = 0; r < 4; ++r) ud[r] = u[r] * de[r];
+                    if (MODE == FULL) {
+                        const f4 am = lds4(Am + (c * kC + li) * kSP + g4);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) out = mfma(am[r], u[r], out);
+                    }
+#pragma unroll
+                    for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) S[t][r] = ge == 0.f ? 0.f : ge * S[t][r];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int t = 0; t < DKT; ++t) S[t] = mfma(kc[r * KP + 16 * t], ud[r], S[t]);
                 }
-#pragma unroll
-                for (int t = 0; t < DKT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[t][r] = ge == 0.f ? 0.f : ge * S[t][r];
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int t = 0; t < DKT; ++t) S[t] = mfma(kc[r * KP + 16 * t], ud[r], S[t]);
                 if (MODE == FULL) {
                     E* oc = o + (tc + g4) * so;
                     if (mine && tc + kC <= p.T) {
@@ -645,7 +722,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     float* Zm = Bm + kC * kSP;                  // Z + Z^T
     float* redb = Zm + kC * kSP;                // [2][4][NW][16] by wave: dbeta; dg's pairs (waves 0 and 1), terms of s, terms of j
     float* dotb = redb + 2 * 4 * NW * 16;       // [2][NW]: <dS_C, S0>
-    ChunkTiles* tiles = reinterpret_cast<ChunkTiles*>(dotb + 2 * NW);       // [2]
+    int* oddb = reinterpret_cast<int*>(dotb + 2 * NW);                      // [2] (of 4): not all of a chunk's results are finite
+    ChunkTiles* tiles = reinterpret_cast<ChunkTiles*>(oddb + 4);            // [2]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g4 = (lane >> 4) << 2;
     const long long bh = blockIdx.x, b = bh / p.H;
@@ -765,7 +843,89 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         for (int w = 0; w < TPW; ++w)
             state_load_all(dS[w], rs, soff[w], srow);
     }
+    // The chunk token by token, all waves together (see "values that are not finite"): results over those that are there, and dS anew.
+    auto walk = [&](int c) {
+        const long long t0 = (long long)c * kC;
+        const int n = valid_of(c);
+        const float* Ks = Kb + (c & 1) * kC * KP;
+        const float* Qs = Qb + (c & 1) * kC * KP;
+        const float* Os = Ob + (c & 1) * kC * VP;
+        const ChunkVec& cv = tiles[c & 1].cv;
+        static_assert(TPW == 1, "one tile of value columns a wave");
+        const int col = wave * 16 + li;
+        const bool mine = col < p.DV;
+        float* part = dSs;                      // [2][NW][DKP]: dq, dk by wave; the space of d(state), which is taken first
+        float* sums = redb + (c & 1) * 4 * NW * 16;             // [2][NW]: dbeta, dg
+        if (wave < DVT) {
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dS[0][t][r] = dSs[(16 * t + g4 + r) * VP + col];
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = n - 1; i >= 0; --i) {
+            const float* kt = Ks + i * KP + g4;
+            const float* qt = Qs + i * KP + g4;
+            const E* pv = v + t0 * p.sv[0] + (mine ? col : 0);
+            float db = 0.f, dg = 0.f;
+            fetch_state(c);
+#pragma unroll 1
+            for (int j = 0; j < i; ++j) {
+                const float x = mine ? Elem<E>::get(pv[j * p.sv[0]]) : 0.f;
+                token_decay(S0[0], cv, j);
+                token_add(S0[0], Ks + j * KP + g4, cv.beta[j] * (x - token_dot(S0[0], Ks + j * KP + g4)));
+            }
+            token_decay(S0[0], cv, i);
+            const float be = cv.beta[i], d = mine ? Os[i * VP + col] : 0.f;
+            const float rr = (mine ? Elem<E>::get(pv[i * p.sv[0]]) : 0.f) - token_dot(S0[0], kt), u = be * rr;
+            token_add(dS[0], qt, d);
+            const float du = token_dot(dS[0], kt), dr = be * du;
+#pragma unroll
+            for (int t = 0; t < DKT; ++t) {
+                const f4 x = lds4(kt + 16 * t);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float a = row_sum(mine ? (S0[0][t][r] + x[r] * u) * d : 0.f);
+                    const float b = row_sum(mine ? dS[0][t][r] * u - S0[0][t][r] * dr : 0.f);
+                    if (li == 0) { part[wave * DKP + 16 * t + g4 + r] = a; part[(NW + wave) * DKP + 16 * t + g4 + r] = b; }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            token_add(dS[0], kt, -dr);
+#pragma unroll
+            for (int t = 0; t < DKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) dg += mine && 16 * t + g4 + r < p.DK ? dS[0][t][r] * S0[0][t][r] : 0.f;
+            db = row_sum(mine ? du * rr : 0.f);
+            dg = wave_sum(dg);
+            if (lane == 0) { sums[wave] = db; sums[NW + wave] = dg; }
+            if (mine && g4 == 0) (reinterpret_cast<E*>(p.dv) + ((t0 + i) * st + bh) * p.DV)[col] = Elem<E>::put(dr);
+            token_decay(dS[0], cv, i);
+            __syncthreads();
+            for (int e = threadIdx.x; e < p.DK; e += 64 * NW) {
+                float a = 0.f, b = 0.f;
+                for (int w = 0; w < NW; ++w) { a += part[w * DKP + e]; b += part[(NW + w) * DKP + e]; }
+                const long long at = ((t0 + i) * st + bh) * p.DK + e;
+                if (p.dq32) {
+                    p.dq32[at] = a;
+                    p.dk32[at] = b;
+                } else {
+                    reinterpret_cast<E*>(p.dq)[at] = Elem<E>::put(a);
+                    reinterpret_cast<E*>(p.dk)[at] = Elem<E>::put(b);
+                }
+            }
+            if (threadIdx.x == 0) {
+                float a = 0.f, b = 0.f;
+                for (int w = 0; w < NW; ++w) { a += sums[w]; b += sums[NW + w]; }
+                p.dbeta[(t0 + i) * st + bh] = a;
+                p.dg[(t0 + i) * st + bh] = cv.seg[i] < 0.f ? 0.f : b;
+            }
+            __syncthreads();
+        }
+    };
     const int last = cend - 1;
+    if (threadIdx.x < 2) oddb[threadIdx.x] = 0;
     if (last >= cbeg) {
         fetch_rows(last);
         commit_rows(last);
@@ -835,6 +995,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
                 y = mfma(ct.Ti[(g4 + r) * kSP + li], kd[r], y);
                 nu = mfma(nm[r], u[r], nu);
             }
+            if (__any(not_finite(u) + not_finite(y) != 0.f) && lane == 0) oddb[par] = 1;
             E* dv = reinterpret_cast<E*>(p.dv) + ((t0 + g4) * st + bh) * p.DV + col;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -868,6 +1029,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             if (li == 0) red[wave * 16 + g4 + r] = db[r];
         }
         __syncthreads();
+        if (threadIdx.x == 0) oddb[par ^ 1] = 0;        // (all have read it before this barrier; the next chunk writes it behind the next)
         if (wave < 2) {         // wave 0: do U^T, wave 1: X U^T
             const float* ar = (wave == 0 ? Os : Xs) + li * VP + g4;
             const float* ur = Us + li * VP + g4;
@@ -981,6 +1143,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             if (li == 0) { red[(2 * NW + wave) * 16 + g4 + r] = ps[r]; red[(3 * NW + wave) * 16 + g4 + r] = pj[r]; }
         }
         __syncthreads();
+        if (__builtin_expect(oddb[par], 0)) {
+            walk(c);
+            if (c > cbeg) fetch_state(c - 1);
+            continue;
+        }
         if (wave == 0) {        // (the others go on: red, dotb and the tiles alternate)
             float sb = 0.f, ws = 0.f, wj = 0.f, dot = 0.f;
 #pragma unroll
@@ -1214,7 +1381,7 @@ int fwd_typed(const Seq& p, hipStream_t st) {
 template <typename E, int DKT, int DVT, int NW, bool VEC>
 int launch_bwd(const Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, VP = DVT * 16 + 4;
-    const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 8 * NW * 16 + 2 * NW) + 2 * sizeof(ChunkTiles);
+    const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 8 * NW * 16 + 2 * NW + 4) + 2 * sizeof(ChunkTiles);
     if (!allow_lds(delta_bwd_k<E, DKT, DVT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_bwd: shared memory refused");
     hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3((unsigned)(p.B * p.H), p.nseg), dim3(64 * NW), lds, st, p);
     return done("dcc_delta_bwd");

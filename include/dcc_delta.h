@@ -16,8 +16,10 @@
  * head h reads key head h / (H / HK).  g (log decay, <= 0 in use), beta: [T, B, H] float32; masks: [T, B] float32 or NULL (no restarts).
  * The last axis of q, k, v, do is contiguous, the others have strides in ELEMENTS (st_*: t, b, h); so have g, beta (t, b, h) and
  * masks (t, b).  States are contiguous [B, H, DK, DV] float32 and stay in 32 bits.  1 <= DK, DV <= DCC_DELTA_MAX_DIM.
- * exp(g_t) that is 0 in float32 restarts the state like a mask.  Non-finite inputs reach every output of the 16-token chunk they lie
- * in (chunks start at t = 0, 16, ...), the later tokens of their sequence up to the next restart after that chunk, and nothing else.
+ * exp(g_t) that is 0 in float32 restarts the state like a mask.  Values that are not finite reach what the recurrence, taken token by token,
+ * lets them reach: the results of their token and of later ones up to the next restart, the gradients of earlier ones down to the last
+ * restart (a chunk of 16 tokens that holds such values takes many times as long).  Finite ones whose sums leave float32's range may reach
+ * their whole chunk (chunks start at t = 0, 16, ...).
  *
  * All pointers are device pointers; calls are asynchronous on `stream` and keep nothing; return 0 or a negative DCC_E* code with
  * the message in dcc_last_error().  T == 0 or B == 0 launch nothing except the copy of the state.  Results do not depend on
