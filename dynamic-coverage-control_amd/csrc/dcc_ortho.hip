@@ -11,7 +11,9 @@
 // Large products over X are C = A B^T of bf16 planes: fp32 MFMA has 1/16 of the bf16 rate, so a value is kept as the sum of bf16 parts
 // and the products of the parts are accumulated in float32.  float32 and float16 matrices take three parts (x = hi + mid + lo to
 // 24 bits) and the six products hh, hm, mh, hl, lh, mm; what is dropped is below 2^-26 of a product.  bfloat16 matrices take two parts and
-// hh, hm, mh (2^-17 of a product: 1/64 of the half step that the result is rounded by).
+// hh, hm, mh (2^-17 of a product), with X itself kept in float32: X <- a X + (b A + c A^2) X, the first term without a product.  The errors of
+// the products are of either sign and average out over their depth: 1e-5 to 3e-5 of the result after five steps, where float32 products
+// leave 3e-6 to 3e-5.  (X in two parts, with a X among the products, left 8e-5 to 6e-4: its own rounding does not average out.)
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
@@ -612,6 +614,7 @@ __device__ __forceinline__ long long plane_at(long long row, int k, int s, long 
 struct Split {                          // planes of the scaled X [R][C]: as it lies (`same` [rp][cp]) and / or transposed (`turned` [cp][rp])
     const void* x;
     ushort_t *same, *turned;
+    float* whole;                       // and the scaled X in float32, [rp][cp] (or null)
     int R, C, rp, cp, tcols;     // padded to kTile with zeros
     Scale s;
 };
@@ -641,6 +644,7 @@ __global__ __launch_bounds__(256) void ortho_split_k(const SplitBatch bt) {
         split<NP>(v[q], h);
 #pragma unroll
         for (int s = 0; s < NP; ++s) {
+            if (s == 0 && p.whole) p.whole[(long long)(i0 + r0 * 16 + q) * p.cp + j0 + c] = v[q];
             if (p.same) p.same[plane_at<NP>(i0 + r0 * 16 + q, j0 + c, s, p.cp)] = h[s];
             if (p.turned) sh[s][c][r0 * 16 + q] = h[s];
         }
@@ -660,10 +664,11 @@ struct Gemm {                           // v = alpha A B^T + beta E + diag I
     const ushort_t *a, *b, *e;          // planes; rows of A and B are contiguous over the depth
     ushort_t *d1, *d2;                  // planes of v as [i][j] and as [j][i] (either may be null)
     void* out;                          // or, bounded by rows and cols, v itself
+    float* x;                           // two parts: v += xa x, and x = v unless out is given; [i][j] or, xt, [j][i]
     long long ldo;                      // row length of out
     int lda, ldb, lde, ld1, ld2, K,     // depths of the planes' rows; of this product
-         rows, cols, dto, sym, tcols, tiles;
-    float alpha, beta, diag;
+         rows, cols, dto, sym, tcols, tiles, ldx, xt;
+    float alpha, beta, diag, xa;
 };
 using GemmBatch = Batch<Gemm>;
 
@@ -805,6 +810,23 @@ __global__ __launch_bounds__(512) void ortho_gemm_k(const GemmBatch bt) {
         multiply(f1);
     }
     __syncthreads();
+    f4 whole[NP == 2 ? 4 : 1][2];
+    if constexpr (NP == 2) {            // (padded like the planes: no bounds)
+        if (p.x) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const long long i = i0 + wi + 16 * x + g4, j = j0 + wj + 16 * y + li;
+                    if (p.xt) {
+                        whole[x][y] = *reinterpret_cast<const f4*>(p.x + j * p.ldx + i);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) whole[x][y][r] = p.x[(i + r) * p.ldx + j];
+                    }
+                }
+        }
+    }
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -815,6 +837,7 @@ __global__ __launch_bounds__(512) void ortho_gemm_k(const GemmBatch bt) {
                 float v = acc[x][y][r];
                 if constexpr (NP == 3) v += low[x][y][r];
                 v *= p.alpha;
+                if constexpr (NP == 2) v += p.x ? p.xa * whole[x][y][r] : 0.f;
                 if (p.e) {
                     float e = 0.f;
 #pragma unroll
@@ -827,6 +850,22 @@ __global__ __launch_bounds__(512) void ortho_gemm_k(const GemmBatch bt) {
             }
         }
     if (p.out) return;
+    if constexpr (NP == 2) {
+        if (p.x) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const long long i = i0 + wi + 16 * x + g4, j = j0 + wj + 16 * y + li;
+                    if (p.xt) {
+                        *reinterpret_cast<f4*>(p.x + j * p.ldx + i) = acc[x][y];
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) p.x[(i + r) * p.ldx + j] = acc[x][y][r];
+                    }
+                }
+        }
+    }
     // planes leave through LDS, whole rows at a time
     constexpr int kRow = kTile + 8;
     ushort_t* sh = reinterpret_cast<ushort_t*>(lds);
@@ -935,7 +974,7 @@ int planes_of(int dtype) { return dtype == DCC_ORTHO_BF16 ? 2 : 3; }
 int norm_blocks(const dcc_ortho_mat& t) { return (int)std::max<int64_t>(1, std::min<int64_t>(kNormBlocks, t.M * t.N / 4096)); }
 
 // where a matrix's intermediate results lie in the workspace
-struct Place { int64_t norm, A, B, W, Q0, Q1, Xp, Xt0, Xt1, X0, X1, part, end; };
+struct Place { int64_t norm, A, B, W, Q0, Q1, Xp, Xt0, Xt1, X0, X1, whole, part, end; };
 Place place_of(const Shape& s, int dtype, int steps, int64_t at) {
     Place p = {};
     auto take = [&](int64_t bytes) { const int64_t o = at; at += up(bytes, kAlign); return o; };
@@ -951,6 +990,7 @@ Place place_of(const Shape& s, int dtype, int steps, int64_t at) {
         p.A = take(np2 * mp * mp); p.B = take(np2 * mp * mp);
         p.Xp = take(np2 * mp * np); p.Xt0 = take(np2 * np * mp);
         if (steps > 1) p.Xt1 = take(np2 * np * mp);
+        if (planes_of(dtype) == 2) p.whole = take(4 * mp * np);
     }
     p.end = at;
     return p;
@@ -1204,6 +1244,8 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
             Split sp = {};
             sp.x = t.in; sp.R = (int)t.M; sp.C = (int)t.N; sp.rp = s.tall ? np : mp; sp.cp = s.tall ? mp : np;
             sp.same = s.tall ? Xt[0] : Xp; sp.turned = s.tall ? Xp : Xt[0];
+            float* whole = np2 == 2 ? reinterpret_cast<float*>(ws + pl.whole) : nullptr;
+            sp.whole = whole;
             sp.tcols = sp.cp / 64; sp.s = Scale{norm, 1, nb, eps};
             round(r++).split[np2 - 2].push_back(sp);
             int cur = 0;
@@ -1213,11 +1255,12 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
                 g.a = g.b = Xp; g.lda = g.ldb = np; g.K = np; g.rows = g.cols = m; g.sym = 1; g.alpha = 1.f;
                 g.d1 = g.d2 = A; g.ld1 = g.ld2 = mp; g.tcols = mp / kTile;
                 round(r++).gemm[np2 - 2].push_back(g);
-                Gemm p = g;             // B = a I + b A + c A^2
-                p.a = p.b = p.e = A; p.lda = p.ldb = p.lde = mp; p.K = mp; p.d1 = p.d2 = B; p.alpha = c; p.beta = b; p.diag = a;
+                Gemm p = g;             // B = a I + b A + c A^2, with two parts without a I
+                p.a = p.b = p.e = A; p.lda = p.ldb = p.lde = mp; p.K = mp; p.d1 = p.d2 = B; p.alpha = c; p.beta = b; p.diag = whole ? 0.f : a;
                 round(r++).gemm[np2 - 2].push_back(p);
-                Gemm q = {};            // X <- B X
+                Gemm q = {};            // X <- B X (+ a X)
                 q.K = q.lda = q.ldb = mp; q.alpha = 1.f;
+                q.x = whole; q.xa = a; q.ldx = sp.cp; q.xt = s.tall && left > 0;
                 if (left == 0) {
                     q.a = s.tall ? Xt[cur] : B; q.b = s.tall ? B : Xt[cur];
                     q.rows = (int)t.M; q.cols = (int)t.N; q.out = t.out; q.ldo = t.N; q.dto = dtype;

@@ -911,9 +911,9 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 def orthogonalize(mats, steps=5, coeffs=NEWTON_SCHULZ, eps=1e-7, out=None):
     """Newton-Schulz orthogonalisation of every matrix of a list (a tensor [M,N], [..,M,N] or a list of such), as the Muon optimiser
-    takes it: X = G / (|G|_F + eps), transposed when M > N; `steps` times X <- (a I + b A + c A^2) X with A = X X^T, coeffs = (a, b, c).
-    Contiguous float32 / bfloat16 / float16 device tensors of one type; `out`: tensors like them, apart from them (allocated when
-    None).  -> the results, as a tensor or a list like `mats`.  No gradient.  No CPU path."""
+    takes it: X = G / (|G|_F + eps), transposed when M > N; `steps` times X <- (a I + b A + c A^2) X with A = X X^T, coeffs = (a, b, c)
+    (they and eps as float32).  Contiguous float32 / bfloat16 / float16 device tensors of one type; `out`: tensors like them, apart from
+    them (allocated when None).  -> the results, as a tensor or a list like `mats`.  No gradient.  No CPU path."""
     single = torch.is_tensor(mats)
     ms = [mats] if single else list(mats)
     outs = None if out is None else ([out] if single else list(out))

@@ -10,7 +10,7 @@
  * for every matrix of the list, all matrices of the list together in each launch (a network has a handful of small ones).
  * For small m and for n much longer than m the steps are taken on the m x m side in float64, which is the same polynomial of X in another
  * order.  Large, nearly square matrices are taken step by step: float32 and float16 in products of 24 bits summed in float32, bfloat16 in
- * products of 16 bits (1/64 of the half step that the result is rounded by) summed in float32.  The norm is summed in float64, so any
+ * products of 16 bits on a float32 X (3e-5 of the result or less, like float32 throughout).  The norm is summed in float64, so any
  * finite G has one; G == 0 gives 0.
  *
  * Calls are asynchronous on `stream`, use only `workspace`, keep nothing, and return 0 or a negative DCC_E* code with the message in
