@@ -108,7 +108,8 @@ __device__ __forceinline__ double inverse_norm(const Scale& s, double* red, doub
     v = 0.;
     for (int w = 0; w < (int)blockDim.x / 64; ++w) v += red[w];
     if (note && threadIdx.x == 0) *note = v;
-    return 1. / (sqrt(v) + (double)s.eps);
+    v = sqrt(v) + (double)s.eps;
+    return v == 0. ? 0. : 1. / v;       // (X == 0 without an eps stays 0)
 }
 
 struct NormMat { const void* x; double* out; long long n; int blocks; };
@@ -628,7 +629,7 @@ __global__ __launch_bounds__(256) void ortho_split_k(const SplitBatch bt) {
     const Split& p = bt.p[pi];
     const E* x = reinterpret_cast<const E*>(p.x);
     const int blk = blockIdx.x - bt.first[pi], i0 = blk / p.tcols * 64, j0 = blk % p.tcols * 64;
-    const float inv = (float)inverse_norm(p.s, red);
+    const double inv = inverse_norm(p.s, red);          // (in float32 it may be subnormal or infinite where the products are neither)
     const int c = threadIdx.x & 63, r0 = threadIdx.x >> 6;
     const int jc = j0 + c < p.C ? j0 + c : p.C - 1;
     float v[16];
@@ -636,7 +637,7 @@ __global__ __launch_bounds__(256) void ortho_split_k(const SplitBatch bt) {
     for (int q = 0; q < 16; ++q) {
         const int i = i0 + r0 * 16 + q, ic = i < p.R ? i : p.R - 1;
         v[q] = get(x[(long long)ic * p.C + jc]);
-        v[q] = i < p.R && j0 + c < p.C ? v[q] * inv : 0.f;
+        v[q] = i < p.R && j0 + c < p.C ? (float)(v[q] * inv) : 0.f;
     }
 #pragma unroll
     for (int q = 0; q < 16; ++q) {
