@@ -691,7 +691,7 @@ template <int NP> constexpr int kAhead = NP == 2 ? 3 : 2;       // (as many as L
 // every load that is under way (2048 x 2048, two parts: 76 us instead of 50), there being no way to tell it which slice a
 // barrier is about.  Nothing but LDS is written, so no register is at stake.
 __device__ __forceinline__ void load_lds(const char* base, unsigned off, unsigned to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
 }
 // this wave's LDS reads and all but its last N loads are done; then all waves meet
 template <int N>
