@@ -74,6 +74,7 @@ struct Seq {        // dcc_delta_seq / dcc_delta_grad as the kernels read them
     float *dg, *dbeta, *dstate0;
     int nseg, seglen;            // the chunks in segments of `seglen` (a multiple of the block) that run side by side; nseg 1: one
     float *sumN, *sumP, *segS;   // [nseg - 1] segment summaries N [DK, DV], P [DK, DK]; [nseg] states at segment starts (all per (row, head))
+    long long first;             // this launch's first (row, head) pair (delta_step_k: first workgroup)
     int vec;        // rows of q, k (and dout, v) may be read four elements at a time
 };
 
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
     float* Am = Qs + BT * kC * KP;              // [BT][16][kSP] (Q K^T) . D
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g4 = (lane >> 4) << 2;
-    const long long bh = blockIdx.x, b = bh / p.H;
+    const long long bh = p.first + blockIdx.x, b = bh / p.H;
     const int h = (int)(bh - b * p.H), hk = h / p.rep;
     const int nt = (p.DV + 15) / 16, tile0 = blockIdx.y * NW + wave;
     // (SUM_BWD leaves out segment 0, the others the last one)
@@ -726,7 +727,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     ChunkTiles* tiles = reinterpret_cast<ChunkTiles*>(oddb + 4);            // [2]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g4 = (lane >> 4) << 2;
-    const long long bh = blockIdx.x, b = bh / p.H;
+    const long long bh = p.first + blockIdx.x, b = bh / p.H;
     const int h = (int)(bh - b * p.H), hk = h / p.rep;
     const E* q = reinterpret_cast<const E*>(p.q) + b * p.sq[1] + hk * p.sq[2];
     const E* k = reinterpret_cast<const E*>(p.k) + b * p.sk[1] + hk * p.sk[2];
@@ -1205,7 +1206,7 @@ __global__ __launch_bounds__(256) void delta_fold_k(const float* __restrict__ a,
 template <typename E, int R, int VEC>
 __global__ __launch_bounds__(256) void delta_step_k(const Seq p, int slices) {
     const int lane = threadIdx.x & 63;
-    const long long w = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long w = (p.first + blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long bh = w / slices;
     if (bh >= p.B * p.H) return;
     const long long b = bh / p.H;
@@ -1344,19 +1345,27 @@ bool allow_lds(K kernel, size_t bytes) {
     return bytes <= 65536 || hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess;
 }
 
+// A launch holds less than 2^32 threads in a direction: n workgroups of at most 512 in as many launches as that takes
+template <typename F>
+int in_launches(Seq& p, int64_t n, const char* what, F launch) {
+    constexpr int64_t kMost = 1 << 22;
+    for (p.first = 0; p.first < n; p.first += kMost) launch((unsigned)std::min(n - (int64_t)p.first, kMost));
+    return done(what);
+}
+
 template <typename E, int DKT, int BT, int NW, bool VEC, int MODE>
-int launch_walk(const Seq& p, hipStream_t st) {
+int launch_walk(Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, TILES = MODE == SUM_FWD ? 1 : 2;
     const size_t lds = sizeof(float) * TILES * (BT * kC * KP + BT * kC * kSP) + BT * sizeof(ChunkVec);
     const int nt = (p.DV + 15) / 16 + (MODE == FULL ? 0 : (p.DK + 15) / 16);
     if (!allow_lds(delta_fwd_k<E, DKT, BT, NW, VEC, MODE>, lds)) return dcc_fail(kEHIP, "gated delta rule: shared memory refused");
-    hipLaunchKernelGGL((delta_fwd_k<E, DKT, BT, NW, VEC, MODE>), dim3((unsigned)(p.B * p.H), (nt + NW - 1) / NW, MODE == FULL ? p.nseg : p.nseg - 1),
-                       dim3(64 * NW), lds, st, p);
-    return done("gated delta rule");
+    return in_launches(p, p.B * p.H, "gated delta rule", [&](unsigned pairs) {
+        hipLaunchKernelGGL((delta_fwd_k<E, DKT, BT, NW, VEC, MODE>), dim3(pairs, (nt + NW - 1) / NW, MODE == FULL ? p.nseg : p.nseg - 1), dim3(64 * NW), lds, st, p);
+    });
 }
 // segment summaries and the states at the segments' starts (dir SUM_FWD) or ends (SUM_BWD)
 template <typename E, int DKT, int DIR>
-int segments(const Seq& p, hipStream_t st) {
+int segments(Seq& p, hipStream_t st) {
     const int rc = p.vec ? launch_walk<E, DKT, 4, 4, true, DIR>(p, st) : launch_walk<E, DKT, 1, 4, false, DIR>(p, st);
     if (rc != 0) return rc;
     const dim3 grid((unsigned)(p.B * p.H), (p.DV + 15) / 16);
@@ -1365,7 +1374,7 @@ int segments(const Seq& p, hipStream_t st) {
     return done("gated delta rule");
 }
 template <typename E, int DKT>
-int fwd_dk(const Seq& p, hipStream_t st) {
+int fwd_dk(Seq& p, hipStream_t st) {
     if (p.nseg > 1)
         if (const int rc = segments<E, DKT, SUM_FWD>(p, st)) return rc;
     if (!p.vec) return launch_walk<E, DKT, 1, 4, false, FULL>(p, st);
@@ -1373,21 +1382,22 @@ int fwd_dk(const Seq& p, hipStream_t st) {
     return p.DV <= 32 ? launch_walk<E, DKT, 2, 2, true, FULL>(p, st) : launch_walk<E, DKT, 4, 4, true, FULL>(p, st);
 }
 template <typename E>
-int fwd_typed(const Seq& p, hipStream_t st) {
+int fwd_typed(Seq& p, hipStream_t st) {
     const int t = (p.DK + 15) / 16;
     return t <= 2 ? fwd_dk<E, 2>(p, st) : t <= 4 ? fwd_dk<E, 4>(p, st) : fwd_dk<E, 8>(p, st);
 }
 
 template <typename E, int DKT, int DVT, int NW, bool VEC>
-int launch_bwd(const Seq& p, hipStream_t st) {
+int launch_bwd(Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, VP = DVT * 16 + 4;
     const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 8 * NW * 16 + 2 * NW + 4) + 2 * sizeof(ChunkTiles);
     if (!allow_lds(delta_bwd_k<E, DKT, DVT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_bwd: shared memory refused");
-    hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3((unsigned)(p.B * p.H), p.nseg), dim3(64 * NW), lds, st, p);
-    return done("dcc_delta_bwd");
+    return in_launches(p, p.B * p.H, "dcc_delta_bwd", [&](unsigned pairs) {
+        hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3(pairs, p.nseg), dim3(64 * NW), lds, st, p);
+    });
 }
 template <typename E, int DKT>
-int bwd_dv(const Seq& p, hipStream_t st) {
+int bwd_dv(Seq& p, hipStream_t st) {
     const int t = (p.DV + 15) / 16;
     constexpr int NW = DKT > 4 ? 8 : 4;
     if (p.nseg > 1)
@@ -1396,7 +1406,7 @@ int bwd_dv(const Seq& p, hipStream_t st) {
     return t <= 2 ? launch_bwd<E, DKT, 2, NW, true>(p, st) : t <= 4 ? launch_bwd<E, DKT, 4, NW, true>(p, st) : launch_bwd<E, DKT, 8, 8, true>(p, st);
 }
 template <typename E>
-int bwd_typed(const Seq& p, hipStream_t st) {
+int bwd_typed(Seq& p, hipStream_t st) {
     const int t = (p.DK + 15) / 16;
     const int rc = t <= 2 ? bwd_dv<E, 2>(p, st) : t <= 4 ? bwd_dv<E, 4>(p, st) : bwd_dv<E, 8>(p, st);
     if (rc != 0 || !p.dq32) return rc;
@@ -1426,17 +1436,17 @@ bool step_overlaps(const dcc_delta_seq* s) {
     return meet(o, s0) || meet(o, s1) || (s->state1 != s->state0 && meet(s1, s0));
 }
 template <typename E, int R>
-int step_rows(const Seq& p, hipStream_t st) {
+int step_rows(Seq& p, hipStream_t st) {
     // four columns per lane where the state's rows allow it; one where that would leave the chip empty (under 1024 waves)
     const bool vec = p.DV % 4 == 0 && aligned(p.state0, 16) && aligned(p.state_out, 16) && p.B * p.H * ((p.DV + 63) / 64) >= 1024;
     const int slices = vec ? (p.DV + 63) / 64 : (p.DV + 15) / 16;
-    const long long blocks = (p.B * p.H * slices + 3) / 4;
-    if (vec) hipLaunchKernelGGL((delta_step_k<E, R, 4>), dim3((unsigned)blocks), dim3(256), 0, st, p, slices);
-    else hipLaunchKernelGGL((delta_step_k<E, R, 1>), dim3((unsigned)blocks), dim3(256), 0, st, p, slices);
-    return done("dcc_delta_step");
+    return in_launches(p, (p.B * p.H * slices + 3) / 4, "dcc_delta_step", [&](unsigned blocks) {
+        if (vec) hipLaunchKernelGGL((delta_step_k<E, R, 4>), dim3(blocks), dim3(256), 0, st, p, slices);
+        else hipLaunchKernelGGL((delta_step_k<E, R, 1>), dim3(blocks), dim3(256), 0, st, p, slices);
+    });
 }
 template <typename E>
-int step_typed(const Seq& p, hipStream_t st) {
+int step_typed(Seq& p, hipStream_t st) {
     return p.DK <= 32 ? step_rows<E, 8>(p, st) : p.DK <= 64 ? step_rows<E, 16>(p, st) : p.DK <= 96 ? step_rows<E, 24>(p, st) : step_rows<E, 32>(p, st);
 }
 
@@ -1509,7 +1519,7 @@ DCC_API int dcc_delta_step(const dcc_delta_seq* s, void* stream) {
     if (s->B == 0) return 0;
     if (!s->q || !s->k || !s->v || !s->g || !s->beta || !s->o || !s->state0 || !s->state1) return refuse("dcc_delta_step", "null pointer");
     if (step_overlaps(s)) return refuse("dcc_delta_step", "o and state1 must lie apart from the operands and from each other (state1 may be state0)");
-    const Seq p = base(s);
+    Seq p = base(s);
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     switch (s->dtype) {
         case DCC_DELTA_F32: return step_typed<float>(p, st);

@@ -689,7 +689,8 @@ template <int NP> constexpr int kAhead = NP == 2 ? 3 : 2;       // (as many as L
 
 // 16 bytes a lane from base + off to LDS bytes to + 16 * lane.  Written out, and with it the waits: the compiler's own barrier waits for
 // every load that is under way (2048 x 2048, two parts: 76 us instead of 50), there being no way to tell it which slice a
-// barrier is about.  Nothing but LDS is written, so no register is at stake.
+// barrier is about.  Nothing but LDS and m0 is written.  m0 is reserved (it can't be declared): the compiler keeps nothing in it between
+// instructions, and sets it right before each that reads it, of which this kernel has no other.
 __device__ __forceinline__ void load_lds(const char* base, unsigned off, unsigned to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
 }
