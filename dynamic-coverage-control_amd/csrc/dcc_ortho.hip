@@ -1040,13 +1040,20 @@ bool outputs_meet(const dcc_ortho_mat* mats, const std::vector<int>& live, int64
     }
     return false;
 }
-// calls f with batches of at most kMaxProds of `all` and their numbers of blocks and descriptions
+// calls f with batches of at most kMaxProds of `all` and their numbers of blocks and descriptions; what makes a launch larger than kMaxBlocks
+// (of up to 512 threads: a launch holds less than 2^32) begins the next
+constexpr int64_t kMaxBlocks = 1 << 22;
 template <typename P, typename Blocks, typename F>
 void batches(const std::vector<P>& all, Blocks blocks, F f) {
-    for (size_t from = 0; from < all.size(); from += kMaxProds) {
+    for (size_t from = 0, to; from < all.size(); from = to) {
         Batch<P> bt;
-        const int n = (int)std::min<size_t>(kMaxProds, all.size() - from);
-        for (int i = 0; i < n; ++i) bt.p[i] = all[from + i];
+        int64_t held = 0;
+        for (to = from; to < all.size() && to < from + kMaxProds; ++to) {
+            held += blocks(all[to]);
+            if (to > from && held > kMaxBlocks) break;
+            bt.p[to - from] = all[to];
+        }
+        const int n = (int)(to - from);
         const unsigned sum = number(bt, n, blocks);
         f(bt, sum, n);
     }
