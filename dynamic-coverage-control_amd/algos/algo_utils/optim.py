@@ -131,21 +131,29 @@ class FlatAdam(torch.optim.Optimizer):
                 "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}
 
     def load_state_dict(self, sd):
+        """This optimizer's own state, or (FlatAdam) that of a torch.optim.Adam.  Anything else is refused with nothing changed."""
         if sd.get("format") == self.FORMAT:
             if sd["numels"] != [p.numel() for p in self._params]:
-                raise ValueError("FlatAdam.load_state_dict: parameter layout differs")
+                raise ValueError("%s.load_state_dict: parameter layout differs" % type(self).__name__)
             self.exp_avg.copy_(sd["exp_avg"]); self.exp_avg_sq.copy_(sd["exp_avg_sq"])
             self.step_count = int(sd["step"])
             for g, sg in zip(self.param_groups, sd["param_groups"]):
                 g.update({k: v for k, v in sg.items() if k != "params"})
             return
-        if "format" in sd:
-            raise ValueError("%s.load_state_dict: the checkpoint holds the state of another optimizer (%s)" % (type(self).__name__, sd["format"]))
+        # (without a format: a torch.optim.Adam's, in the order that FlatAdam keeps; FlatMuon reorders, and its exp_avg is no average)
+        if "format" in sd or self.FORMAT != FlatAdam.FORMAT:
+            raise ValueError("%s.load_state_dict: the checkpoint holds the state of another optimizer (%s)"
+                             % (type(self).__name__, sd.get("format", "torch.optim.Adam")))
         # a torch.optim.Adam state_dict (checkpoints written before the flat optimizer): per-parameter moments
         state, groups = sd["state"], sd["param_groups"]
         ids = [i for g in groups for i in g["params"]]
         if len(ids) != len(self._params):
             raise ValueError("FlatAdam.load_state_dict: %d parameters in the checkpoint, %d here" % (len(ids), len(self._params)))
+        for i, p in zip(ids, self._params):
+            for m in ("exp_avg", "exp_avg_sq") if state.get(i) is not None else ():
+                if state[i][m].shape != p.shape:
+                    raise ValueError("FlatAdam.load_state_dict: parameter %s is %s here, its %s in the checkpoint %s"
+                                     % (i, tuple(p.shape), m, tuple(state[i][m].shape)))
         self.exp_avg.zero_(); self.exp_avg_sq.zero_()
         step = 0
         for i, p, off in zip(ids, self._params, self._offsets):
