@@ -335,9 +335,9 @@ class Learner:
         E, N = r_buffer.n_rollout_threads, self.n_agents
         masks = (1.0 - out["done"].to(torch.float32)).view(E, 1, 1).expand(E, N, 1)
         rewards = out["reward"].view(E, 1, 1).expand(E, N, 1)
-        if rnn_a is not None:      # GRU states of finished envs restart from zero (learner.py:258-265)
-            keep = masks.reshape(E, N, 1, 1)
-            rnn_a, rnn_c = rnn_a * keep, rnn_c * keep
+        if rnn_a is not None:      # states of finished envs restart from zero (learner.py:258-265), whatever they held: 0 * NaN is NaN
+            done = masks.reshape(E, N, 1, 1) == 0
+            rnn_a, rnn_c = rnn_a.masked_fill(done, 0.0), rnn_c.masked_fill(done, 0.0)
         r_buffer.insert(None, None, rnn_a, rnn_c, actions, action_log_probs, values, rewards, masks)
 
     @torch.no_grad()

@@ -1,0 +1,23 @@
+"""States of the recurrent policies on their way through learner and buffer: restarts are selected, and a buffer that cannot fit says so."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+NAN, INF = float("nan"), float("inf")
+
+
+def test_a_finished_env_restarts_whatever_its_state_held():
+    from learner import Learner
+    E, N, L, S = 3, 2, 1, 5
+    rnn_a, rnn_c = torch.randn(E, N, L, S), torch.randn(E, N, L, S)
+    rnn_a[1, 0, 0, 2], rnn_c[1, 1, 0, 0], rnn_c[1, 0, 0, 1] = NAN, INF, -INF
+    kept = []
+    buf = SimpleNamespace(n_rollout_threads=E, insert=lambda *a: kept.append(a))
+    done = torch.tensor([0, 1, 0], dtype=torch.uint8)
+    Learner.insert(SimpleNamespace(n_agents=N), ({"done": done, "reward": torch.zeros(E)}, None, None, None, rnn_a, rnn_c), buf)
+    a, c, masks = kept[0][2], kept[0][3], kept[0][-1]
+    assert (a[1] == 0).all() and (c[1] == 0).all()
+    for e in (0, 2):
+        assert torch.equal(a[e], rnn_a[e]) and torch.equal(c[e], rnn_c[e])
+    assert masks.shape == (E, N, 1) and float(masks[1].sum()) == 0 and float(masks.sum()) == (E - 1) * N
