@@ -119,6 +119,19 @@ class _Rows(object):
         return getattr(self._full(), name)
 
 
+def recurrent_state_bytes(T, E, N, layers, size):
+    """Bytes of the recurrent states that a buffer keeps: every step's and the last, of actor and critic."""
+    return 2 * (T + 1) * E * N * layers * size * 4
+
+
+def check_state_memory(need, have):
+    """Refuses states that alone are more than the device holds, before torch runs out of memory somewhere else."""
+    if need > have:
+        raise ValueError("the recurrent states of every step take %.1f GB (actor and critic) and the device has %.1f GB: fewer "
+                         "n_rollout_threads, a shorter max_ep_len, or (recurrent_core: gated_delta) smaller delta_heads / delta_head_dim"
+                         % (need / 1e9, have / 1e9))
+
+
 class SharedReplayBuffer(object):
     def __init__(self, cfg, obs_space, cent_obs_space, act_space, device=None, compact=False, n_pois=None,
                  expander=None, featurizer=None):
@@ -187,6 +200,9 @@ class SharedReplayBuffer(object):
         self.recurrent = bool(cfg.use_recurrent_policy or cfg.use_naive_recurrent_policy)
         if self.recurrent and self.store_state:
             raise ValueError("recurrent policies read observation rows: use structured_input: false, compact_obs: false")
+        if self.recurrent and torch.device(self.device).type == "cuda":
+            check_state_memory(recurrent_state_bytes(T, E, N, cfg.recurrent_N, state_size(cfg)),
+                               torch.cuda.get_device_properties(self.device).total_memory)
         self.rnn_states = z(T + 1, E, N, cfg.recurrent_N, state_size(cfg) if self.recurrent else 0)
         self.rnn_states_critic = torch.zeros_like(self.rnn_states)
         self.available_actions = None

@@ -21,3 +21,14 @@ def test_a_finished_env_restarts_whatever_its_state_held():
     for e in (0, 2):
         assert torch.equal(a[e], rnn_a[e]) and torch.equal(c[e], rnn_c[e])
     assert masks.shape == (E, N, 1) and float(masks[1].sum()) == 0 and float(masks.sum()) == (E - 1) * N
+
+
+def test_states_that_cannot_fit_are_refused_by_name():
+    """the buffer keeps every step's state, twice; 4096 envs of 8 agents with 4 heads of 64 x 64 need 648 GB and one card has 288"""
+    from buffer.shared_buffer import check_state_memory, recurrent_state_bytes
+    one = 151 * 4096 * 8 * 1 * 4 * 64 * 64 * 4
+    assert recurrent_state_bytes(150, 4096, 8, 1, 4 * 64 * 64) == 2 * one
+    with pytest.raises(ValueError, match="648.5 GB.*delta_head_dim"):
+        check_state_memory(2 * one, 288 * 10 ** 9)
+    check_state_memory(recurrent_state_bytes(150, 4096, 8, 1, 4 * 32 * 32), 288 * 10 ** 9)       # 162 GB: the default heads
+    check_state_memory(recurrent_state_bytes(150, 4096, 8, 1, 256), 288 * 10 ** 9)
