@@ -1010,6 +1010,12 @@ const char* list_error(const dcc_ortho_mat* mats, int32_t count, int32_t dtype, 
     return nullptr;
 }
 
+// do two arrays of n floats share bytes?
+bool meet(const float* a, const float* b, int64_t n) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), len = (uintptr_t)n * 4;
+    return x < y + len && y < x + len;
+}
+
 // numbers the workgroups of a batch's n descriptions: returns how many there are
 template <typename P, typename Blocks>
 unsigned number(Batch<P>& bt, int n, Blocks blocks) {
@@ -1316,6 +1322,7 @@ DCC_API int dcc_muon_momentum(const float* grad, float* buf, float* dir, int64_t
     if (!grad || !buf || !dir || n < 1) return dcc_fail(kEINVAL, "dcc_muon_momentum: null pointer or n < 1");
     if ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(buf) | reinterpret_cast<uintptr_t>(dir)) & 15)
         return dcc_fail(kEINVAL, "dcc_muon_momentum: arrays must be 16-byte aligned");
+    if (meet(grad, buf, n) || meet(grad, dir, n) || meet(buf, dir, n)) return dcc_fail(kEINVAL, "dcc_muon_momentum: arrays must lie apart");
     const int64_t nb = std::min<int64_t>(((n >> 2) + 3 + 255) / 256, 2048);
     hipLaunchKernelGGL(muon_momentum_k, dim3((unsigned)nb), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), grad, buf, dir, (long long)n, momentum,
                        nesterov, clip);
@@ -1329,6 +1336,9 @@ DCC_API int dcc_muon_apply(float* param, const float* dir, const dcc_muon_seg* s
     for (int i = 0; i < count; ++i)
         if (segs[i].offset < 0 || segs[i].offset % 4 || segs[i].numel < 0 || segs[i].numel > (1ll << 40))
             return dcc_fail(kEINVAL, "dcc_muon_apply: a range must start at a multiple of 4 and hold 0..2^40 elements");
+    int64_t end = 0;
+    for (int i = 0; i < count; ++i) end = std::max(end, segs[i].offset + segs[i].numel);
+    if (meet(param, dir, end)) return dcc_fail(kEINVAL, "dcc_muon_apply: param and dir must lie apart");
     for (int from = 0; from < count; from += kMaxSegs) {
         Segs s;
         s.count = 0;

@@ -771,11 +771,18 @@ def grad_norm_clip(flat_grad, max_norm, out, workspace):
                                                  _stream()), "dcc_grad_norm_clip")
 
 
+def check_clip(what, clip, device):
+    """clip: None, or the scale of the gradient as a float32 number on `device` (what grad_norm_clip leaves)."""
+    if clip is not None and not (torch.is_tensor(clip) and clip.dtype == torch.float32 and clip.device == device and clip.numel() >= 1):
+        raise ValueError("%s: clip must be None or a float32 number on %s" % (what, device))
+
+
 def adam_step(param, grad, exp_avg, exp_avg_sq, step_size, bc2_sqrt, beta1, beta2, eps, weight_decay, clip=None):
     for t, nm in ((param, "param"), (grad, "grad"), (exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq")):
         _f32c(t, nm)
         if t.numel() != param.numel():
             raise ValueError("adam_step: %s has %d elements, param %d" % (nm, t.numel(), param.numel()))
+    check_clip("adam_step", clip, param.device)
     with torch.cuda.device(param.device):
         _check(load_library().dcc_adam_step(_ptr(param), _ptr(grad), _ptr(exp_avg), _ptr(exp_avg_sq), param.numel(), float(step_size),
                                             float(bc2_sqrt), float(beta1), float(beta2), float(eps), float(weight_decay),
@@ -951,11 +958,13 @@ def orthogonalize(mats, steps=5, coeffs=NEWTON_SCHULZ, eps=1e-7, out=None):
 
 
 def muon_momentum(grad, buf, direction, momentum, nesterov=True, clip=None):
-    """buf = momentum * buf + clip * grad; direction = clip * grad + momentum * buf (nesterov) or buf, on flat float32 arrays."""
+    """buf = momentum * buf + clip * grad; direction = clip * grad + momentum * buf (nesterov) or buf, on flat float32 arrays
+    that lie apart; clip: None or a float32 number on their device."""
     for t, nm in ((grad, "grad"), (buf, "buf"), (direction, "direction")):
         _f32c(t, nm)
         if t.numel() != grad.numel() or t.device != grad.device:
             raise ValueError("muon_momentum: %s has %d elements on %s, grad %d on %s" % (nm, t.numel(), t.device, grad.numel(), grad.device))
+    check_clip("muon_momentum", clip, grad.device)
     with _on(grad):
         _check(load_library().dcc_muon_momentum(_ptr(grad), _ptr(buf), _ptr(direction), grad.numel(), float(momentum), int(bool(nesterov)),
                                                 _ptr(clip), _stream()), "dcc_muon_momentum")

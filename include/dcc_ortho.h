@@ -51,7 +51,7 @@ DCC_API int64_t dcc_ortho_workspace_bytes(const dcc_ortho_mat* mats, int32_t cou
 DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t dtype, int32_t steps, float a, float b, float c,
                               float eps, void* workspace, void* stream);
 
-/* The two element-wise ends of a Muon step on flat float32 arrays (16-byte aligned):
+/* The two element-wise ends of a Muon step on flat float32 arrays (16-byte aligned, apart from each other):
  *   dcc_muon_momentum   g = clip * grad;  buf = momentum * buf + g;  dir = nesterov ? g + momentum * buf : buf
  *                       (clip: device pointer to the scale of the gradient, NULL = 1; dcc_grad_norm_clip leaves it)
  *   dcc_muon_apply      param = keep * param - segs[i].scale * dir on every range of the list (ranges must not overlap) */
