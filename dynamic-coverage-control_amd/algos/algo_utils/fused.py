@@ -342,10 +342,13 @@ def gated_delta(q, k, v, g, beta, state=None, masks=None, scale=None):
         S' = m_t exp(g_t) S;   u = beta_t (v_t - S'^T k_t);   S = S' + k_t u^T;   o_t = scale * S^T q_t
     q, k [T,B,HK,DK], v [T,B,H,DV] (value head h reads key head h // (H // HK)), g, beta [T,B,H], state [B,H,DK,DV] or None (zero),
     masks [T,B] or None (0: the state restarts from zero before that token).  -> o [T,B,H,DV], last state [B,H,DK,DV].
-    On the GPU float32 / bfloat16 / float16 q, k, v with float32 g, beta, state run the HIP kernels."""
+    On the GPU float32 / bfloat16 / float16 q, k, v with float32 g, beta, state run the HIP kernels; other types run in torch."""
     if q.dim() != 4 or v.dim() != 4:
         raise ValueError("gated_delta: q, k are [T,B,HK,DK] and v is [T,B,H,DV]")
     scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    if v.is_cuda and v.dtype in (torch.float32, torch.bfloat16, torch.float16) and not torch.is_autocast_enabled():
+    if (v.is_cuda and v.dtype in (torch.float32, torch.bfloat16, torch.float16) and not torch.is_autocast_enabled()
+            and all(x is None or x.dtype == torch.float32 for x in (g, beta, state))):
+        if masks is not None and masks.dtype != torch.float32:
+            masks = (masks != 0).float()
         return _GatedDelta.apply(q, k, v, g, beta, state, masks, scale)
     return _gated_delta_torch(q, k, v, g, beta, state, masks, scale)

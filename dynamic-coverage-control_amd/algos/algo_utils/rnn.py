@@ -92,7 +92,7 @@ class GatedDeltaLayer(nn.Module):
             g = -torch.exp(self.A_log[i]) * F.softplus(a + self.dt_bias[i])
             beta = torch.sigmoid(b)
             S = hxs[:, i].reshape(B, H, D, D)
-            if T == 1 and x.is_cuda and not torch.is_grad_enabled() and not torch.is_autocast_enabled():
+            if T == 1 and x.is_cuda and x.dtype == torch.float32 and not torch.is_grad_enabled() and not torch.is_autocast_enabled():
                 import dcc_hip
                 o, S = dcc_hip.gated_delta_step(q[0], k[0], v[0], g[0], beta[0], S.contiguous(), m[0])
             else:
