@@ -1335,9 +1335,9 @@ Seq base(const dcc_delta_seq* s) {
 }
 int done(const char* what) {
     const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string(what) + ": " + hipGetErrorString(e));
+    return e == hipSuccess ? 0 : dcc_fail_nothrow(kEHIP, what, ": ", hipGetErrorString(e));
 }
-int refuse(const char* what, const char* why) { return dcc_fail(kEINVAL, std::string(what) + ": " + why); }
+int refuse(const char* what, const char* why) { return dcc_fail_nothrow(kEINVAL, what, ": ", why); }
 
 // a workgroup may ask for more than the 64 KB that a launch allows by itself (a CU has 160)
 template <typename K>
@@ -1358,7 +1358,7 @@ int launch_walk(Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, TILES = MODE == SUM_FWD ? 1 : 2;
     const size_t lds = sizeof(float) * TILES * (BT * kC * KP + BT * kC * kSP) + BT * sizeof(ChunkVec);
     const int nt = (p.DV + 15) / 16 + (MODE == FULL ? 0 : (p.DK + 15) / 16);
-    if (!allow_lds(delta_fwd_k<E, DKT, BT, NW, VEC, MODE>, lds)) return dcc_fail(kEHIP, "gated delta rule: shared memory refused");
+    if (!allow_lds(delta_fwd_k<E, DKT, BT, NW, VEC, MODE>, lds)) return dcc_fail_nothrow(kEHIP, "gated delta rule: shared memory refused");
     return in_launches(p, p.B * p.H, "gated delta rule", [&](unsigned pairs) {
         hipLaunchKernelGGL((delta_fwd_k<E, DKT, BT, NW, VEC, MODE>), dim3(pairs, (nt + NW - 1) / NW, MODE == FULL ? p.nseg : p.nseg - 1), dim3(64 * NW), lds, st, p);
     });
@@ -1391,7 +1391,7 @@ template <typename E, int DKT, int DVT, int NW, bool VEC>
 int launch_bwd(Seq& p, hipStream_t st) {
     constexpr int KP = DKT * 16 + 4, VP = DVT * 16 + 4;
     const size_t lds = sizeof(float) * (4 * kC * KP + 4 * kC * VP + DKT * 16 * VP + 2 * kC * kSP + 8 * NW * 16 + 2 * NW + 4) + 2 * sizeof(ChunkTiles);
-    if (!allow_lds(delta_bwd_k<E, DKT, DVT, NW, VEC>, lds)) return dcc_fail(kEHIP, "dcc_delta_bwd: shared memory refused");
+    if (!allow_lds(delta_bwd_k<E, DKT, DVT, NW, VEC>, lds)) return dcc_fail_nothrow(kEHIP, "dcc_delta_bwd: shared memory refused");
     return in_launches(p, p.B * p.H, "dcc_delta_bwd", [&](unsigned pairs) {
         hipLaunchKernelGGL((delta_bwd_k<E, DKT, DVT, NW, VEC>), dim3(pairs, p.nseg), dim3(64 * NW), lds, st, p);
     });

@@ -1151,21 +1151,21 @@ DCC_API int64_t dcc_ortho_workspace_bytes(const dcc_ortho_mat* mats, int32_t cou
 
 DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t dtype, int32_t steps, float a, float b, float c,
                               float eps, void* workspace, void* stream) try {
-    if (const char* e = list_error(mats, count, dtype, steps)) return dcc_fail(kEINVAL, std::string("dcc_orthogonalize: ") + e);
-    if (!(eps >= 0.f)) return dcc_fail(kEINVAL, "dcc_orthogonalize: eps must not be negative");
+    if (const char* e = list_error(mats, count, dtype, steps)) return dcc_fail_nothrow(kEINVAL, "dcc_orthogonalize: ", e);
+    if (!(eps >= 0.f)) return dcc_fail_nothrow(kEINVAL, "dcc_orthogonalize: eps must not be negative");
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const int64_t esize = dtype == DCC_ORTHO_F32 ? 4 : 2;
     std::vector<int> live;
     for (int i = 0; i < count; ++i) {
         if (mats[i].M == 0 || mats[i].N == 0) continue;
-        if (!mats[i].in || !mats[i].out) return dcc_fail(kEINVAL, "dcc_orthogonalize: null matrix");
+        if (!mats[i].in || !mats[i].out) return dcc_fail_nothrow(kEINVAL, "dcc_orthogonalize: null matrix");
         if ((reinterpret_cast<uintptr_t>(mats[i].in) | reinterpret_cast<uintptr_t>(mats[i].out)) & (esize - 1))
-            return dcc_fail(kEINVAL, "dcc_orthogonalize: a matrix is not aligned to its elements");
+            return dcc_fail_nothrow(kEINVAL, "dcc_orthogonalize: a matrix is not aligned to its elements");
         live.push_back(i);
     }
     if (live.empty()) return 0;
-    if (outputs_meet(mats, live, esize)) return dcc_fail(kEINVAL, "dcc_orthogonalize: an output overlaps an input or another output");
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))) return dcc_fail(kEINVAL, "dcc_orthogonalize: workspace must be 256-byte aligned");
+    if (outputs_meet(mats, live, esize)) return dcc_fail_nothrow(kEINVAL, "dcc_orthogonalize: an output overlaps an input or another output");
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & (kAlign - 1))) return dcc_fail_nothrow(kEINVAL, "dcc_orthogonalize: workspace must be 256-byte aligned");
     char* ws = reinterpret_cast<char*>(workspace);
 
     // every matrix's products, round by round; a round's products (of all matrices) run together
@@ -1309,36 +1309,36 @@ DCC_API int dcc_orthogonalize(const dcc_ortho_mat* mats, int32_t count, int32_t 
                 hipLaunchKernelGGL(ortho_square_k<1>, dim3(all), dim3(64 * kWaves), 0, st, fine);
             }
         });
-        if (!launch_gemm<2>(q.gemm[0], st) || !launch_gemm<3>(q.gemm[1], st)) return dcc_fail(kEHIP, "dcc_orthogonalize: shared memory refused");
+        if (!launch_gemm<2>(q.gemm[0], st) || !launch_gemm<3>(q.gemm[1], st)) return dcc_fail_nothrow(kEHIP, "dcc_orthogonalize: shared memory refused");
     }
     const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string("dcc_orthogonalize: ") + hipGetErrorString(e));
+    return e == hipSuccess ? 0 : dcc_fail_nothrow(kEHIP, "dcc_orthogonalize: ", hipGetErrorString(e));
 } catch (...) {
-    return dcc_fail(kEINVAL, "dcc_orthogonalize: out of host memory");
+    return dcc_fail_nothrow(kEINVAL, "dcc_orthogonalize: out of host memory");
 }
 
 DCC_API int dcc_muon_momentum(const float* grad, float* buf, float* dir, int64_t n, float momentum, int32_t nesterov, const float* clip,
                               void* stream) {
-    if (!grad || !buf || !dir || n < 1) return dcc_fail(kEINVAL, "dcc_muon_momentum: null pointer or n < 1");
+    if (!grad || !buf || !dir || n < 1) return dcc_fail_nothrow(kEINVAL, "dcc_muon_momentum: null pointer or n < 1");
     if ((reinterpret_cast<uintptr_t>(grad) | reinterpret_cast<uintptr_t>(buf) | reinterpret_cast<uintptr_t>(dir)) & 15)
-        return dcc_fail(kEINVAL, "dcc_muon_momentum: arrays must be 16-byte aligned");
-    if (meet(grad, buf, n) || meet(grad, dir, n) || meet(buf, dir, n)) return dcc_fail(kEINVAL, "dcc_muon_momentum: arrays must lie apart");
+        return dcc_fail_nothrow(kEINVAL, "dcc_muon_momentum: arrays must be 16-byte aligned");
+    if (meet(grad, buf, n) || meet(grad, dir, n) || meet(buf, dir, n)) return dcc_fail_nothrow(kEINVAL, "dcc_muon_momentum: arrays must lie apart");
     const int64_t nb = std::min<int64_t>(((n >> 2) + 3 + 255) / 256, 2048);
     hipLaunchKernelGGL(muon_momentum_k, dim3((unsigned)nb), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), grad, buf, dir, (long long)n, momentum,
                        nesterov, clip);
     const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string("dcc_muon_momentum: ") + hipGetErrorString(e));
+    return e == hipSuccess ? 0 : dcc_fail_nothrow(kEHIP, "dcc_muon_momentum: ", hipGetErrorString(e));
 }
 
 DCC_API int dcc_muon_apply(float* param, const float* dir, const dcc_muon_seg* segs, int32_t count, float keep, void* stream) {
-    if (count < 0 || !param || !dir || (count > 0 && !segs)) return dcc_fail(kEINVAL, "dcc_muon_apply: null pointer or negative count");
-    if ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(dir)) & 15) return dcc_fail(kEINVAL, "dcc_muon_apply: arrays must be 16-byte aligned");
+    if (count < 0 || !param || !dir || (count > 0 && !segs)) return dcc_fail_nothrow(kEINVAL, "dcc_muon_apply: null pointer or negative count");
+    if ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(dir)) & 15) return dcc_fail_nothrow(kEINVAL, "dcc_muon_apply: arrays must be 16-byte aligned");
     for (int i = 0; i < count; ++i)
         if (segs[i].offset < 0 || segs[i].offset % 4 || segs[i].numel < 0 || segs[i].numel > (1ll << 40))
-            return dcc_fail(kEINVAL, "dcc_muon_apply: a range must start at a multiple of 4 and hold 0..2^40 elements");
+            return dcc_fail_nothrow(kEINVAL, "dcc_muon_apply: a range must start at a multiple of 4 and hold 0..2^40 elements");
     int64_t end = 0;
     for (int i = 0; i < count; ++i) end = std::max(end, segs[i].offset + segs[i].numel);
-    if (meet(param, dir, end)) return dcc_fail(kEINVAL, "dcc_muon_apply: param and dir must lie apart");
+    if (meet(param, dir, end)) return dcc_fail_nothrow(kEINVAL, "dcc_muon_apply: param and dir must lie apart");
     for (int from = 0; from < count; from += kMaxSegs) {
         Segs s;
         s.count = 0;
@@ -1350,11 +1350,11 @@ DCC_API int dcc_muon_apply(float* param, const float* dir, const dcc_muon_seg* s
             first += (segs[i].numel + 4095) / 4096;
             ++s.count;
         }
-        if (first > 2147483647) return dcc_fail(kEINVAL, "dcc_muon_apply: more than 2^43 elements in one list");
+        if (first > 2147483647) return dcc_fail_nothrow(kEINVAL, "dcc_muon_apply: more than 2^43 elements in one list");
         if (s.count) hipLaunchKernelGGL(muon_apply_k, dim3((unsigned)first), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), param, dir, s);
     }
     const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? 0 : dcc_fail(kEHIP, std::string("dcc_muon_apply: ") + hipGetErrorString(e));
+    return e == hipSuccess ? 0 : dcc_fail_nothrow(kEHIP, "dcc_muon_apply: ", hipGetErrorString(e));
 }
 
 }  // extern "C"
