@@ -339,10 +339,10 @@ __device__ __forceinline__ void token_decay(f4 (&S)[T], const ChunkVec& cv, int 
 // own start.  SUM_BWD does the same for d(state), which runs the other way: dS <- gam_C dS + Q^T (gam do) - K^T (gam X) needs no state.
 //
 // Bound by the issue of instructions in chains of small products, with two to four waves a SIMD.  8192 (row, head) pairs of 150 tokens,
-// 64 x 64 float32, with checkpoints: 850 us, 2.7 GB at 3.2 TB/s, fp32 MFMA busy a third of the time.  8 heads of 16384 tokens, 128 x 128
-// bfloat16: 190 us in 32 segments and 245 us for their summaries, where one after the other they would take some 6 ms.  Blocks of four chunks
+// 64 x 64 float32, with checkpoints: 800 - 830 us, 2.9 GB at 3.5 TB/s, fp32 MFMA busy 37 % of the time.  8 heads of 16384 tokens, 128 x 128
+// bfloat16: 190 - 205 us in 32 segments and 250 - 265 us for their summaries, where one after the other they would take some 6 ms.  Blocks of four chunks
 // against one: the preparation of a chunk is a chain of 5 us for one wave, and four waves do one each; a sequence of one chunk takes the
-// block of one (960 x 4 pairs of 10 tokens: 65 us, 145 MB).
+// block of one (960 x 4 pairs of 10 tokens: 59 us, 220 MB).
 enum { FULL = 0, SUM_FWD = 1, SUM_BWD = 2 };
 
 template <typename E, int DKT, int BT, int NW, bool VEC, int MODE>
@@ -703,9 +703,9 @@ __global__ __launch_bounds__(64 * DKT) void delta_join_k(const Seq p, int back) 
 // q.dq - v.dv, would have no digits of it left.)  S0 comes from the checkpoints of the forward pass; U, X, dS pass through LDS where the contraction changes from key to value columns.  Between the two
 // halves, waves 0 and 1 form do U^T and X U^T while waves 2 and 3 prepare the state-free part of the chunk that comes next; its rows were
 // loaded one chunk ahead.  Three barriers per chunk.
-// Bound by the chains between those barriers: two workgroups a compute unit (LDS: 67 KB at 64 x 64), 28 thousand cycles a chunk, of which the
-// first half 12, the preparation of the next chunk 7 and the second half 5; waits for memory are below 1.  8192 pairs of 150 tokens, 64 x 64
-// float32: 2.1 ms, 3.6 GB, fp32 MFMA busy a third of the time.  (Two more waves that only prepare leave room for one workgroup: 2.6 ms.)
+// Bound by the chains between those barriers, with two workgroups a compute unit (LDS: 68 KB at 64 x 64) and some 30 thousand cycles a chunk, of
+// which waits for memory are below 1.  8192 pairs of 150 tokens, 64 x 64 float32: 2.0 - 2.1 ms, 4.8 GB, fp32 MFMA busy 34 % of the time.  (Two
+// more waves that only prepare leave room for one workgroup: 2.6 ms.)
 struct ChunkTiles { float Ti[kC * kSP], Am[kC * kSP], Nm[kC * kSP], Dm[kC * kSP]; ChunkVec cv; };
 
 template <typename E, int DKT, int DVT, int NW, bool VEC>
@@ -1200,8 +1200,8 @@ __global__ __launch_bounds__(256) void delta_fold_k(const float* __restrict__ a,
 }
 
 // ---- one token -----------------------------------------------------------------------------------------------------------------
-// Bound by reading and writing the state once: 32768 x 4 states of 64 x 64 in 835 us, 5.3 TB/s, where a large copy reaches 4.7; 1000 x 6 states
-// of 96 x 80 in 70 us.  64 x 4 states take 4.5 us.  A wave owns one (row, head) and 16 * VEC value columns; lane l holds columns
+// Bound by reading and writing the state once: 32768 x 4 states of 64 x 64 in 845 us, 5.2 TB/s, where a large copy reaches 4.8 and an addition in
+// place 5.9; 1000 x 6 states of 96 x 80 in 70 us.  64 x 4 states take 4.5 us.  A wave owns one (row, head) and 16 * VEC value columns; lane l holds columns
 // VEC * (l % 16).. of the key rows 4 i + l / 16, all of them loaded before the first use.
 template <typename E, int R, int VEC>
 __global__ __launch_bounds__(256) void delta_step_k(const Seq p, int slices) {

@@ -186,7 +186,7 @@ __device__ __forceinline__ void mirror(double* out, int mq, int i, int j, double
 
 // Short depths: a 32 x 32 tile per workgroup of eight waves, each of which takes every eighth run of 16 of the depth for the whole tile
 // (latency counts: a wave's loads are all under way together, and its chain of products is short); the partial tiles are added in LDS.
-// A product of 256 x 256 takes 5.5 us in a launch of its own (launch, two loads one after the other, 16 MFMA, LDS, store), 1 us of it MFMA.
+// A product of 256 x 256 takes 6.4 us and more in a launch of its own (median 7.6) (launch, two loads one after the other, 16 MFMA, LDS, store), 1 us of it MFMA.
 constexpr int kWaves = 8;
 struct Tile32 { d4 t[2][2]; };
 template <typename FA, typename FB>
@@ -958,8 +958,9 @@ struct Shape { int64_t m, n; bool tall; };
 Shape shape_of(const dcc_ortho_mat& t) { return Shape{std::min(t.M, t.N), std::max(t.M, t.N), t.M > t.N}; }
 
 // The m x m side in float64: always up to 704, where a product's 32 x 32 tiles (253) have a compute unit each (600 x 700, five steps: 258 us
-// here, step by step 508 in float32 and 317 in bfloat16), above it where X is long enough.  1000 x 2500 float32: 907 and 902 us,
-// 1000 x 5000: 1048 and 1457, 2048 x 8192: 6225 and 3442; bfloat16: 1000 x 5000 1062 and 779, 1000 x 10000 1298 and 1248.
+// here, step by step 508 in float32 and 317 in bfloat16; 704 x 704 and 705 x 705: 282 and 344 in bfloat16), above it where X is long enough.
+// 1000 x 2500 float32: 907 and 902 us,
+// 1000 x 5000: 1042 and 1457, 2048 x 8192: 6225 and 3419; bfloat16: 1000 x 5000 1062 and 812, 1000 x 10000 1289 and 1330.
 bool on_square_side(const Shape& s, int dtype) { return s.m <= 704 || s.n >= s.m * s.m / (dtype == DCC_ORTHO_BF16 ? 100 : 256); }
 constexpr int kGroup = 5;               // steps on that side before X X^T is formed anew
 // X <- Q X in tiles of 64 x 128 where they fill the chip twice (256 x 32768: 226 us in all, in tiles of 32 x 32 284; 256 x 4096: 134 and 128)

@@ -21,6 +21,8 @@
  * restart (a chunk of 16 tokens that holds such values takes many times as long).  Finite ones whose sums leave float32's range may reach
  * their whole chunk (chunks start at t = 0, 16, ...).
  *
+ * Results lie apart from the operands and from each other (but for a step's state in place).
+ *
  * All pointers are device pointers; calls are asynchronous on `stream` and keep nothing; return 0 or a negative DCC_E* code with
  * the message in dcc_last_error().  T == 0 or B == 0 launch nothing except the copy of the state.  Results do not depend on
  * scheduling: no atomics.
