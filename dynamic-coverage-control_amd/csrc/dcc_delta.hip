@@ -73,6 +73,7 @@ struct Seq {        // dcc_delta_seq / dcc_delta_grad as the kernels read them
     void *dq, *dk, *dv;
     float *dg, *dbeta, *dstate0;
     int nseg, seglen;            // the chunks in segments of `seglen` (a multiple of the block) that run side by side; nseg 1: one
+    int* cuts;                   // [nseg - 1] does the summarised segment hold a restart?
     float *sumN, *sumP, *segS;   // [nseg - 1] segment summaries N [DK, DV], P [DK, DK]; [nseg] states at segment starts (all per (row, head))
     long long first;             // this launch's first (row, head) pair (delta_step_k: first workgroup)
     int vec;        // rows of q, k (and dout, v) may be read four elements at a time
@@ -292,9 +293,9 @@ __device__ __forceinline__ void chunk_products(const float* kr, const float* qr,
 
 // ---- values that are not finite ------------------------------------------------------------------------------------------------
 // The products of a chunk meet every token with every other: what is not finite would reach tokens before it and tokens behind a restart,
-// by way of 0 * NaN.  A chunk whose results are not all finite is therefore taken again, token by token: these are its pieces, for a lane's
-// part of a state, rows 16 t + 4 * (lane / 16) + r of one column.  (Anything in the inputs that is not finite shows in the results: every
-// update of a chunk is a sum over all its tokens.)  The barriers to the scheduler keep the registers of these rare paths few.
+// by way of 0 * NaN.  Where a chunk holds such values, what they reach is taken token by token instead: forward and in the summaries, by
+// column, the tokens that they reach; in the gradient, the whole chunk.  These are its pieces, for a lane's part of a state, rows 16 t + 4 *
+// (lane / 16) + r of one column.  The barriers to the scheduler keep the registers of these rare paths few.
 __device__ __forceinline__ float not_finite(const f4& x) { return (x[0] * 0.f + x[1] * 0.f) + (x[2] * 0.f + x[3] * 0.f); }      // 0, or NaN
 template <int T>
 __device__ __forceinline__ float token_dot(const f4 (&S)[T], const float* row) {         // S^T row; row: LDS, at + 4 * (lane / 16)
@@ -345,8 +346,9 @@ __device__ __forceinline__ void token_decay(f4 (&S)[T], const ChunkVec& cv, int 
 // block of one (960 x 4 pairs of 10 tokens: 59 us, 220 MB).
 enum { FULL = 0, SUM_FWD = 1, SUM_BWD = 2 };
 
+// (waves a SIMD: what the loop itself has room for; the rare path must not take it)
 template <typename E, int DKT, int BT, int NW, bool VEC, int MODE>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4 ? 2 : 3))) void delta_fwd_k(const Seq p) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu((DKT > 4 ? 2 : DKT > 2 && BT > 1 ? 3 : 4) + (DKT > 2 && MODE == SUM_FWD && BT > 1 ? 1 : 0)))) void delta_fwd_k(const Seq p) {
     constexpr int DKP = DKT * 16, KP = DKP + 4, CPW = (BT + NW - 1) / NW;
     constexpr bool HASQ = MODE != SUM_FWD;
     extern __shared__ float sh[];
@@ -425,6 +427,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
             vnext[r] = v[(t < p.T ? t : p.T - 1) * sv0];
         }
     };
+    bool cutseg = false;
     const int nblk = (cend - cbeg + BT - 1) / BT;
     auto block = [&](int i) { return cbeg + BT * (MODE == SUM_BWD ? nblk - 1 - i : i); };
     if (nblk > 0) {
@@ -484,9 +487,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
                 const float* kr = Ks + (c * kC + li) * KP + g4;
                 const float* qr = Qs + (c * kC + li) * KP + g4;
                 const ChunkVec& cv = cvs[c];
-                const f4 be = lds4(cv.beta + g4), ga = lds4(cv.gam + g4), de = lds4(cv.toend + g4);
-                const float ge = cv.gend;
-                const int odd = cv.odd;
+                const f4 be = lds4(cv.beta + g4), ga = lds4(cv.gam + g4);
+                f4 de = lds4(cv.toend + g4);
+                float ge = cv.gend;
+                const int odd = __builtin_amdgcn_readfirstlane(cv.odd);
+                if (MODE != FULL) cutseg |= cv.seg[kC - 1] != 0.f;
                 const float* kc = Ks + (c * kC + g4) * KP + li;
                 const float* qc = Qs + (c * kC + g4) * KP + li;
                 f4 ks = zero4(), qs = zero4();
@@ -557,21 +562,44 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
                     rhs[r] = be[r] * (vv[r] - (ga[r] == 0.f ? 0.f : ga[r] * ks[r]));
                     out[r] = ga[r] == 0.f ? 0.f : ga[r] * qs[r];
                 }
-                if (__builtin_expect(odd | __any(not_finite(rhs) != 0.f), 0)) {
-#pragma unroll 1
-                    for (int at = 0; at < valid - c * kC && at < kC; ++at) {
-                        const float* kt = Ks + (c * kC + at) * KP + g4;
-                        const int r = at & 3;
-                        const float x = __shfl(r == 0 ? vv[0] : r == 1 ? vv[1] : r == 2 ? vv[2] : vv[3], 4 * (at - r) + li, 64);
-                        token_decay(S, cv, at);
-                        token_add(S, kt, cv.beta[at] * (x - token_dot(S, kt)));
-                        if (MODE == FULL) {
-                            const float y = token_dot(S, Qs + (c * kC + at) * KP + g4);
+                const bool rare = odd | __any(not_finite(rhs) != 0.f);
+                unsigned met;                   // rare: this lane's tokens that what is not finite reaches, bit r; bit 4: the chunk's end
+                f4 walked;
+                if (__builtin_expect(rare, 0)) {
+                    // By column: what is not finite reaches the tokens from its right-hand side to the end of the stretch between restarts.  They
+                    // and, if the last is among them, the state come from the walk; all else keeps the bits that it has without.  (odd: K, the
+                    // gates or beta are not finite, and all tokens are walked.)
+                    unsigned bad = odd ? 0xffffu : 0u, reach = 0;
+                    walked = zero4();
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) out[e] = g4 + e == at ? y : out[e];
+                    for (int r = 0; r < 4; ++r)
+                        if (rhs[r] * 0.f != 0.f) { bad |= 1u << (g4 + r); rhs[r] = 0.f; }
+                    bad |= __shfl_xor(bad, 16, 64);
+                    bad |= __shfl_xor(bad, 32, 64);
+#pragma unroll 1
+                    for (int at = 0; at < kC; ++at) reach |= ((cv.seg[at] < 0.f ? 0u : reach << 1) | bad) & (1u << at);
+                    met = (reach >> g4 & 15u) | (reach >> 11 & 16u);
+                    if (reach) {
+#pragma unroll 1
+                        for (int at = 0; at < valid - c * kC && at < kC; ++at) {
+                            const float* kt = Ks + (c * kC + at) * KP + g4;
+                            const int r = at & 3;
+                            const float x = __shfl(r == 0 ? vv[0] : r == 1 ? vv[1] : r == 2 ? vv[2] : vv[3], 4 * (at - r) + li, 64);
+                            token_decay(S, cv, at);
+                            token_add(S, kt, cv.beta[at] * (x - token_dot(S, kt)));
+                            if (MODE == FULL) {
+                                const float y = token_dot(S, Qs + (c * kC + at) * KP + g4);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) walked[e] = g4 + e == at ? y : walked[e];
+                            }
                         }
                     }
-                } else {
+                    if (met & 16u) {            // the products leave this state as it is
+                        de = zero4();
+                        ge = 1.f;
+                    }
+                }
+                if (!odd) {
                     const f4 ti = lds4(Ti + (c * kC + li) * kSP + g4);
                     f4 u = zero4();
 #pragma unroll
@@ -593,6 +621,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
 #pragma unroll
                         for (int t = 0; t < DKT; ++t) S[t] = mfma(kc[r * KP + 16 * t], ud[r], S[t]);
                 }
+                if (MODE == FULL && __builtin_expect(rare, 0)) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) out[r] = met >> r & 1u ? walked[r] : out[r];
+                }
                 if (MODE == FULL) {
                     E* oc = o + (tc + g4) * so;
                     if (mine && tc + kC <= p.T) {
@@ -611,6 +643,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DKT > 4
     if (MODE != FULL) {
         const long long at = bh * (p.nseg - 1) + blockIdx.z;
         store_state(unit ? p.sumP + at * p.DK * p.DK : p.sumN + at * sst);
+        if (tile0 == 0 && lane == 0) p.cuts[at] = cutseg;
     } else if (seg == p.nseg - 1) {
         if (p.state_out) store_state(p.state_out + bh * sst);
     }
@@ -628,10 +661,11 @@ __global__ __launch_bounds__(64 * DKT) void delta_join_k(const Seq p, int back) 
     const unsigned srow = 4u * p.DV, off = col < p.DV ? 4u * ((16 * wave + g4) * p.DV + col) : kOutside;
     const int prow = 16 * wave + li;
     // summary i belongs to segment i (forward) or i + 1 (backward)
-    struct Sum { f4 P[DKT], N; };
+    struct Sum { f4 P[DKT], N; int cut; };
     auto fetch = [&](Sum& s, int i) {
         i = back ? n - 1 - i : i;
         i = i < 0 ? 0 : i < n ? i : n - 1;
+        s.cut = p.cuts[bh * n + i];
         const __amdgpu_buffer_rsrc_t rn = state_rsrc(p.sumN + (bh * n + i) * sst, p.DK, p.DV), rp = state_rsrc(p.sumP + (bh * n + i) * spp, p.DK, p.DK);
 #pragma unroll
         for (int r = 0; r < 4; ++r) s.N[r] = state_load(rn, off + r * srow);
@@ -658,13 +692,9 @@ __global__ __launch_bounds__(64 * DKT) void delta_join_k(const Seq p, int back) 
     };
     auto step = [&](const Sum& s, int i) {
         const float (*x)[17] = sh[i & 1];
-        // a segment with a restart has P == 0, and then what the state held before (NaN included) is gone: not multiplied
-        unsigned any = 0;               // (bits: 0 and -0 are zero, NaN is not)
-#pragma unroll
-        for (int t = 0; t < DKT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) any |= __float_as_uint(s.P[t][r]);
-        if (!__any((any & 0x7fffffffu) != 0)) { S = s.N; return; }
+        // behind a restart what the state held before (NaN included) is gone: not multiplied by P == 0.  (P may be 0 by decay alone, which is
+        // no restart: NaN stays NaN.)
+        if (s.cut) { S = s.N; return; }
         f4 a = s.N, c = zero4();
 #pragma unroll
         for (int t = 0; t < DKT; ++t)
@@ -1312,7 +1342,7 @@ int segments_of(const dcc_delta_seq* s, bool backward, int& seglen) {
 }
 int64_t segment_floats(const dcc_delta_seq* s, int nseg) {
     if (nseg <= 1) return 0;
-    return s->B * s->H * ((int64_t)(nseg - 1) * s->DK * (s->DV + s->DK) + (int64_t)nseg * s->DK * s->DV);
+    return s->B * s->H * ((int64_t)(nseg - 1) * (s->DK * (s->DV + s->DK) + 1) + (int64_t)nseg * s->DK * s->DV);
 }
 void place_segments(Seq& p, float* ws) {
     if (p.nseg <= 1) return;
@@ -1320,6 +1350,7 @@ void place_segments(Seq& p, float* ws) {
     p.sumN = ws;
     p.sumP = p.sumN + bh * (p.nseg - 1) * p.DK * p.DV;
     p.segS = p.sumP + bh * (p.nseg - 1) * p.DK * p.DK;
+    p.cuts = reinterpret_cast<int*>(p.segS + bh * p.nseg * p.DK * p.DV);
 }
 Seq base(const dcc_delta_seq* s) {
     Seq p = {};

@@ -172,3 +172,18 @@ def test_the_reference_itself():
     ref = reference(d, 1.0, do, ds)
     assert torch.isnan(ref["o"][3:7, 0, 0]).any() and torch.isfinite(ref["o"][7:]).all() and torch.isfinite(ref["o"][:3]).all()
     assert torch.isfinite(ref["dv"]).all() and torch.isfinite(ref["dq"][:3]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(1100, 1, 1, 3, 32, 40), (1300, 1, 2, 2, 80, 7), (790, 2, 1, 1, 128, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("what,at,restarts", [("v", 3, ()), ("state", None, ()), ("k", 500, ()), ("v", 40, (700,)), ("do", -3, ()), ("dstate", None, ()),
+                                              ("do", -300, (200,))])
+def test_a_long_decay_is_no_restart(size, what, at, restarts):
+    """few rows, many tokens, decays whose product over a segment is 0 in float32: what is not finite stays until a restart, as token by token"""
+    if at is not None and at < 0:
+        at += size[0]
+    d, spoil = place(size, what, NAN, at, restarts, "cuda")
+    d["g"].fill_(-0.7)              # exp(-0.7 * 256) is 0
+    ref = compare(d, size, spoil)
+    if not restarts:
+        assert not torch.isfinite(ref["last" if what in ("v", "state", "k") else "dstate"][0, 0]).all()
