@@ -187,3 +187,35 @@ def test_a_long_decay_is_no_restart(size, what, at, restarts):
     ref = compare(d, size, spoil)
     if not restarts:
         assert not torch.isfinite(ref["last" if what in ("v", "state", "k") else "dstate"][0, 0]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(40, 3, 1, 2, 32, 48), (1100, 1, 1, 2, 64, 20)], ids=lambda s: "x".join(map(str, s)))
+def test_finite_and_not_in_turn_in_a_graph(size):
+    """replays on inputs with and without such values equal the eager calls: nothing of the one is left for the other"""
+    import dcc_hip
+    T, B, HK, H, DK, DV = size
+    sets = [make(*size, reset=0.05, seed=50 + i, device="cuda") for i in range(4)]
+    sets[1]["v"][T // 2, 0, 1, 3], sets[2]["k"][5, 0, 0, 1], sets[2]["state"][0, 1, 2, 2] = NAN, INF, NAN
+    do, ds = torch.randn(T, B, H, DV, device="cuda"), torch.randn(B, H, DK, DV, device="cuda")
+    buf = {n: x.clone() for n, x in sets[0].items()}
+
+    def work(d):
+        o, S, ck = dcc_hip.gated_delta_fwd(*[d[n] for n in NAMES], d["masks"], want_ckpt=True)
+        return [o, S] + list(dcc_hip.gated_delta_bwd(*[d[n] for n in NAMES[:5]], d["masks"], None, ck, do, ds))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        work(buf)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work(buf)
+    for i in (1, 3, 2, 0, 1):
+        for n in buf:
+            buf[n].copy_(sets[i][n])
+        graph.replay()
+        got = [x.clone() for x in outs]
+        torch.cuda.synchronize()
+        for x, y in zip(got, work(sets[i])):
+            assert torch.equal(torch.nan_to_num(x, 7e30), torch.nan_to_num(y, 7e30))

@@ -94,3 +94,29 @@ def test_mixed_list_of_more_than_one_launch(dtype):
     got = dcc_hip.orthogonalize(mats)
     for i, (x, y) in enumerate(zip(mats, got)):
         assert torch.equal(dcc_hip.orthogonalize(x), y), (i, tuple(x.shape))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_step_by_step_in_a_graph(dtype):
+    """captured once, replayed on other matrices with eager calls in between: what a call keeps in its workspace begins anew"""
+    import dcc_hip
+    shapes = [(720, 901), (901, 720), (60, 90)]
+    sets = [[gradient_like(m, n, dtype=dtype, seed=10 * i + j).cuda() for j, (m, n) in enumerate(shapes)] for i in range(3)]
+    buf = [x.clone() for x in sets[0]]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        dcc_hip.orthogonalize(buf)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = dcc_hip.orthogonalize(buf)
+    for i in (1, 2, 1, 0):
+        for x, y in zip(buf, sets[i]):
+            x.copy_(y)
+        graph.replay()
+        got = [x.clone() for x in outs]
+        torch.cuda.synchronize()
+        for x, y in zip(got, dcc_hip.orthogonalize(sets[i])):
+            assert torch.equal(x, y)
